@@ -71,7 +71,8 @@ const char *pgc_status_string(int status);
 int pgc_version(void);
 /* Reads and optionally clears the device error word of the current device: 0 when no kernel
  * recorded a fault, else code + 100 * unit (units: 0 decode and context-parallel exchange,
- * 1 append, 2 copies, 3 prefill, 4 linear attention, 5 q4 projection, 6 prefill projection). Synchronises the device. Replaces the reference's
+ * 1 append, 2 copies, 3 prefill, 4 linear attention, 5 q4 projection, 6 prefill projection,
+ * 7 chunk attention, 8 received-attention weights, 9 cache eviction). Synchronises the device. Replaces the reference's
  * MTLCommandBufferStatusError check at commit time (bridge.m:376). */
 int pgc_device_error(int *code_out, int64_t *detail_out, int clear);
 
@@ -238,6 +239,108 @@ int pgc_prefill_attn(const uint16_t *q, const uint16_t *k_pages, const uint16_t 
                      int64_t num_pages, const int32_t *block_table, int prefix_len,
                      int chunk_len, float scale, uint16_t *out, void *workspace,
                      size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Attention of a ragged batch (no counterpart in the reference, which serves one sequence a call)
+ * ------------------------------------------------------------------------------------- */
+
+#define PGC_CHUNK_MAX_BATCH 4096
+#define PGC_CHUNK_MAX_ROWS (1 << 24)   /* query rows of a call */
+#define PGC_CHUNK_MAX_TOKENS (1 << 24) /* tokens of a sequence */
+
+/* Workspace bytes of pgc_chunk_attn (with_weights = 0) and pgc_chunk_attn_weights (1). Up to
+ * PGC_MAX_QUERIES rows a sequence: the splits' partials, and with weights 16 fp32 scores per query
+ * row and token of max_seq_len. More rows: 37 MiB, and with weights the rows' lse. 0 for shapes that
+ * the entries refuse. */
+size_t pgc_chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_seq_len,
+                                 int with_weights);
+
+/* Causal attention of the new tokens of `batch` sequences over their paged caches, any number of new
+ * tokens a sequence: decode steps, draft verification and prompt chunks of many requests in one
+ * call, with the lengths on the device, so that a captured graph can be replayed with others. The
+ * rows' K/V are in the cache already (pgc_append_kv_rope).
+ *   q          [total_q][16][256] bf16: rotated query rows, the sequences' one after the other
+ *   q_starts   [batch + 1] int32 (device), ascending: sequence b has rows [q_starts[b],
+ *              q_starts[b + 1]), at most max_q_len of them, none allowed
+ *   seq_lens   [batch] int32 (device): tokens in the cache, the new ones included, <= max_seq_len
+ *   block_tables [batch][max_pages_per_seq] int32 (device)
+ *   gate       nullable [total_q][16][256] bf16: out = attn * sigmoid(gate)
+ *   out        [total_q][16][256] bf16
+ *   lse        nullable [total_q][16] fp32: log of the row's sum of exp(scale q.k), before the gate
+ * Row i of a sequence of n rows sits at position seq_lens[b] - n + i and sees the tokens up to it; a
+ * row at a negative position (seq_lens[b] < n) sees nothing: out 0, lse -inf. Rows before q_starts[0]
+ * and from q_starts[batch] on are left as they were. total_q, max_q_len and max_seq_len are
+ * host-side bounds that size the launch: a sequence whose rows break them is skipped, one whose
+ * length does counts as empty, and pgc_device_error reports either. Scores, softmax statistics and
+ * sums are fp32, the probabilities are rounded to bf16 for the P.V product, the output once.
+ * A masked token's score is never used, whatever it is, and slots past a sequence's end are never
+ * read into a sum; but a NaN or infinite V element of a cached token of the sequence makes that output
+ * dim NaN in rows before the token too (its probability there is 0, and 0 times it is NaN).
+ * q, k/v_pages, gate, out and workspace 16-byte aligned. Calls that may overlap on the GPU, and
+ * graphs that may, need workspaces of their own. */
+int pgc_chunk_attn(const uint16_t *q, const uint16_t *k_pages, const uint16_t *v_pages,
+                   int64_t num_pages, const int32_t *block_tables, int max_pages_per_seq,
+                   const int32_t *q_starts, const int32_t *seq_lens, int batch, int total_q,
+                   int max_q_len, int max_seq_len, float scale, const uint16_t *gate, uint16_t *out,
+                   float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
+/* pgc_chunk_attn that also adds, for every cached token, the attention it received:
+ *   weights[slot][h][t] += sum over the sequence's rows that see t and the 4 query heads of kv head h
+ *                          of exp(scale q.k_t - lse)
+ *   weights       [num_slots][4][weights_stride] fp32, weights_stride >= max_seq_len; zeroed by the
+ *                 caller when a sequence starts (pgc_zero_regions)
+ *   slots         nullable [batch] int32 (device): the sequences' slots, distinct; NULL = sequence b
+ *                 uses slot b. A slot out of range or named by an earlier sequence of the batch is
+ *                 recorded (pgc_device_error) and nothing is added for that sequence
+ * Only the tokens [0, seq_lens[b]) of the sequences with rows are touched. The sums' order is fixed:
+ * the same call gives the same bits. */
+int pgc_chunk_attn_weights(const uint16_t *q, const uint16_t *k_pages, const uint16_t *v_pages,
+                           int64_t num_pages, const int32_t *block_tables, int max_pages_per_seq,
+                           const int32_t *q_starts, const int32_t *seq_lens, int batch, int total_q,
+                           int max_q_len, int max_seq_len, float scale, const uint16_t *gate,
+                           uint16_t *out, float *lse, float *weights, int64_t weights_stride,
+                           int64_t num_slots, const int32_t *slots, void *workspace,
+                           size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Eviction from the paged cache by received attention (no counterpart in the reference)
+ * ------------------------------------------------------------------------------------- */
+
+#define PGC_EVICT_MAX_TOKENS 262144 /* longest sequence pgc_kv_evict_select takes */
+
+/* Which tokens each kv head of each sequence keeps. With L = seq_lens[b] <= budget: all. Otherwise
+ * the first keep_first, the last keep_last, and of those between the budget - keep_first - keep_last
+ * with the greatest weights; of equal weights the lowest index, a NaN weight counting as the
+ * smallest.
+ *   weights      [num_slots][4][weights_stride] fp32, as pgc_chunk_attn_weights fills it
+ *   weights_out  nullable, the same shape; may be `weights` itself (otherwise they must not overlap):
+ *                the kept tokens' weights moved to [0, min(L, budget)) of their row and zeros from
+ *                there to L, so that the accumulation goes on over the compacted cache
+ *   slots        as in pgc_chunk_attn_weights
+ *   kept         [batch][4][budget] int32: the kept indices, ascending; -1 behind the last
+ *   new_lens     nullable [batch] int32: min(L, budget); not seq_lens itself
+ * A length outside [0, max_seq_len], or a slot that may not be used, is recorded and the sequence
+ * keeps nothing (kept -1, new_lens 0). budget >= 1, keep_first + keep_last <= budget,
+ * max_seq_len <= PGC_EVICT_MAX_TOKENS, batch <= 65535. */
+int pgc_kv_evict_select(const float *weights, float *weights_out, int64_t weights_stride,
+                        int64_t num_slots, const int32_t *slots, const int32_t *seq_lens, int batch,
+                        int max_seq_len, int budget, int keep_first, int keep_last, int32_t *kept,
+                        int32_t *new_lens, void *stream);
+
+/* Copies the kept K/V rows into the pages of new block tables: for kv head h of sequence b, the row
+ * of token kept[b][h][i] becomes token i; entries < 0 are skipped (their destination rows are left as
+ * they were). The destination pages are the caller's fresh pages (pgc_page_pool_alloc): cached pages
+ * may be shared between sequences, so nothing is moved in place. Source and destination pools may be
+ * the same; the destination pages must not be among the source pages of the call. The keys keep the
+ * rotation of their positions, so decoding goes on with the next position and the new length.
+ *   src_tables [batch][src_max_pages], dst_tables [batch][dst_max_pages] int32 (device),
+ *   dst_max_pages * 16 >= budget. An index past the source table, or a page outside its pool, is
+ *   recorded (pgc_device_error) and the row skipped. Pools 16-byte aligned. */
+int pgc_kv_evict_compact(const uint16_t *src_k_pages, const uint16_t *src_v_pages,
+                         int64_t src_num_pages, const int32_t *src_tables, int src_max_pages,
+                         const int32_t *kept, int batch, int budget, uint16_t *dst_k_pages,
+                         uint16_t *dst_v_pages, int64_t dst_num_pages, const int32_t *dst_tables,
+                         int dst_max_pages, void *stream);
 
 /* ---------------------------------------------------------------------------------------
  * A6-A9, A11: cache copies (prefix snapshot / restore, hidden rows, state)

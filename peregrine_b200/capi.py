@@ -25,6 +25,8 @@ MAX_CONTEXT_TOKENS = 65536
 PARTIAL_FLOATS = HEAD_DIM + 2
 MAX_QUERIES = 4
 MAX_REGIONS = 128
+CHUNK_MAX_BATCH = 4096
+EVICT_MAX_TOKENS = 262144
 APPEND_DECODE = 0
 APPEND_PREFILL = 1
 
@@ -110,6 +112,12 @@ SIGNATURES = {
     "pgc_merge_partials": (I32, [P, I64, I32, I64, P, P, P]),
     "pgc_prefill_workspace_bytes": (SZ, [I32, I32]),
     "pgc_prefill_attn": (I32, [P, P, P, I64, P, I32, I32, F32, P, P, SZ, P]),
+    "pgc_chunk_workspace_bytes": (SZ, [I32, I32, I32, I32, I32]),
+    "pgc_chunk_attn": (I32, [P, P, P, I64, P, I32, P, P, I32, I32, I32, I32, F32, P, P, P, P, SZ, P]),
+    "pgc_chunk_attn_weights": (I32, [P, P, P, I64, P, I32, P, P, I32, I32, I32, I32, F32, P, P, P, P, I64, I64, P,
+                                     P, SZ, P]),
+    "pgc_kv_evict_select": (I32, [P, P, I64, I64, P, P, I32, I32, I32, I32, I32, P, P, P]),
+    "pgc_kv_evict_compact": (I32, [P, P, I64, P, I32, P, I32, I32, P, P, I64, P, I32, P]),
     "pgc_copy_rows": (I32, [P, P, P, P, I64, I64, I64, I64, P]),
     "pgc_kv_restore_dense": (I32, [P, P, I64, I64, P, P, I64, P, I64, I64, I64, P]),
     "pgc_kv_snapshot_dense": (I32, [P, P, I64, P, I64, I64, P, P, I64, I64, I64, P]),
@@ -317,6 +325,50 @@ def prefill_attn(q, k_pages, v_pages, block_table, prefix_len, chunk_len, scale,
         _ptr(q), _ptr(k_pages), _ptr(v_pages), k_pages.shape[0], _ptr(block_table), prefix_len,
         chunk_len, scale, _ptr(out), _ptr(workspace), ws_bytes, _stream(stream)),
         "pgc_prefill_attn")
+
+
+def chunk_workspace_bytes(batch: int, total_q: int, max_q_len: int, max_seq_len: int,
+                          with_weights: bool = False) -> int:
+    return int(lib().pgc_chunk_workspace_bytes(batch, total_q, max_q_len, max_seq_len, int(with_weights)))
+
+
+def chunk_attn(q, k_pages, v_pages, block_tables, q_starts, seq_lens, max_q_len, max_seq_len, scale, out,
+               workspace, gate=None, lse=None, stream=None) -> None:
+    """pgc_chunk_attn: causal attention of a ragged batch; q/out [total_q][16][256], q_starts
+    [batch + 1] and seq_lens [batch] int32 on the device, lse fp32 [total_q][16]."""
+    check(lib().pgc_chunk_attn(
+        _ptr(q), _ptr(k_pages), _ptr(v_pages), k_pages.shape[0], _ptr(block_tables), block_tables.shape[1],
+        _ptr(q_starts), _ptr(seq_lens), seq_lens.shape[0], q.shape[0], max_q_len, max_seq_len, scale, _ptr(gate),
+        _ptr(out), _ptr(lse), _ptr(workspace), workspace.numel() * workspace.element_size(), _stream(stream)),
+        "pgc_chunk_attn")
+
+
+def chunk_attn_weights(q, k_pages, v_pages, block_tables, q_starts, seq_lens, max_q_len, max_seq_len, scale,
+                       out, weights, workspace, gate=None, lse=None, slots=None, stream=None) -> None:
+    """pgc_chunk_attn_weights: chunk_attn that also adds the attention every cached token received to
+    weights fp32 [num_slots][4][stride]; slots [batch] int32."""
+    check(lib().pgc_chunk_attn_weights(
+        _ptr(q), _ptr(k_pages), _ptr(v_pages), k_pages.shape[0], _ptr(block_tables), block_tables.shape[1],
+        _ptr(q_starts), _ptr(seq_lens), seq_lens.shape[0], q.shape[0], max_q_len, max_seq_len, scale, _ptr(gate),
+        _ptr(out), _ptr(lse), _ptr(weights), weights.shape[2], weights.shape[0], _ptr(slots), _ptr(workspace),
+        workspace.numel() * workspace.element_size(), _stream(stream)), "pgc_chunk_attn_weights")
+
+
+def kv_evict_select(weights, seq_lens, max_seq_len, budget, keep_first, keep_last, kept, new_lens=None,
+                    weights_out=None, slots=None, stream=None) -> None:
+    """pgc_kv_evict_select: kept int32 [batch][4][budget] from weights fp32 [num_slots][4][stride]."""
+    check(lib().pgc_kv_evict_select(
+        _ptr(weights), _ptr(weights_out), weights.shape[2], weights.shape[0], _ptr(slots), _ptr(seq_lens),
+        seq_lens.shape[0], max_seq_len, budget, keep_first, keep_last, _ptr(kept), _ptr(new_lens),
+        _stream(stream)), "pgc_kv_evict_select")
+
+
+def kv_evict_compact(src_k, src_v, src_tables, kept, dst_k, dst_v, dst_tables, stream=None) -> None:
+    """pgc_kv_evict_compact: the rows kept int32 [batch][4][budget] into the pages of dst_tables."""
+    check(lib().pgc_kv_evict_compact(
+        _ptr(src_k), _ptr(src_v), src_k.shape[0], _ptr(src_tables), src_tables.shape[1], _ptr(kept),
+        kept.shape[0], kept.shape[2], _ptr(dst_k), _ptr(dst_v), dst_k.shape[0], _ptr(dst_tables),
+        dst_tables.shape[1], _stream(stream)), "pgc_kv_evict_compact")
 
 
 def copy_rows(dst, src, n_rows, row_bytes, dst_pitch, src_pitch, dst_rows=None, src_rows=None,

@@ -221,7 +221,7 @@ int pgc_device_error(int *code_out, int64_t *detail_out, int clear) {
     int st = check_device(nullptr);
     if (st != PGC_OK) return st;
     if (cudaDeviceSynchronize() != cudaSuccess) return PGC_ERR_CUDA;
-    DevErrorHost e[7] = {};
+    DevErrorHost e[10] = {};
     cudaError_t r = decode_read_error(&e[0], clear != 0);
     if (r == cudaSuccess) r = append_read_error(&e[1], clear != 0);
     if (r == cudaSuccess) r = copy_read_error(&e[2], clear != 0);
@@ -229,10 +229,13 @@ int pgc_device_error(int *code_out, int64_t *detail_out, int clear) {
     if (r == cudaSuccess) r = linear_read_error(&e[4], clear != 0);
     if (r == cudaSuccess) r = q4_read_error(&e[5], clear != 0);
     if (r == cudaSuccess) r = prefill_linear_read_error(&e[6], clear != 0);
+    if (r == cudaSuccess) r = chunk_read_error(&e[7], clear != 0);
+    if (r == cudaSuccess) r = chunk_weights_read_error(&e[8], clear != 0);
+    if (r == cudaSuccess) r = evict_read_error(&e[9], clear != 0);
     if (r != cudaSuccess) return PGC_ERR_CUDA;
     int code = 0;
     long long detail = 0;
-    for (int i = 0; i < 7 && code == 0; ++i)
+    for (int i = 0; i < 10 && code == 0; ++i)
         if (e[i].code != 0) {
             code = e[i].code + 100 * i;  // unit in the hundreds digit
             detail = e[i].detail;
@@ -448,6 +451,124 @@ int pgc_prefill_attn(const uint16_t *q, const uint16_t *k_pages, const uint16_t 
     return cuda_status(launch_prefill(q, tk, tv, v_pages, num_pages, block_table, prefix_len, chunk_len,
                                       scale, out, workspace, current_sm_count(),
                                       static_cast<cudaStream_t>(stream)));
+}
+
+// ------------------------------------------------------------------ ragged batches
+static bool chunk_shape_ok(int batch, int total_q, int max_q_len, int max_seq_len) {
+    return batch > 0 && batch <= PGC_CHUNK_MAX_BATCH && total_q > 0 && total_q <= PGC_CHUNK_MAX_ROWS && max_q_len > 0 &&
+           max_seq_len > 0 && max_seq_len <= PGC_CHUNK_MAX_TOKENS;
+}
+
+size_t pgc_chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_seq_len, int with_weights) {
+    if (!chunk_shape_ok(batch, total_q, max_q_len, max_seq_len)) return 0;
+    return chunk_workspace_bytes(batch, total_q, max_q_len, max_seq_len, with_weights != 0, current_sm_count());
+}
+
+static int chunk_call(const uint16_t *q, const uint16_t *k_pages, const uint16_t *v_pages, int64_t num_pages,
+                      const int32_t *block_tables, int max_pages_per_seq, const int32_t *q_starts,
+                      const int32_t *seq_lens, int batch, int total_q, int max_q_len, int max_seq_len,
+                      float scale, const uint16_t *gate, uint16_t *out, float *lse, const ChunkWeights *weights,
+                      void *workspace, size_t workspace_bytes, void *stream) {
+    // arguments are checked before the device is asked for, so refusals need no GPU
+    if (batch < 0 || total_q < 0 || max_q_len < 0 || max_seq_len < 0 || num_pages <= 0 || max_pages_per_seq < 0 ||
+        !std::isfinite(scale))
+        return PGC_ERR_INVALID;
+    if (batch > PGC_CHUNK_MAX_BATCH) return PGC_ERR_BOUNDS;
+    if (weights && (weights->stride < max_seq_len || weights->num_slots <= 0 ||
+                    (!weights->slots && batch > weights->num_slots)))
+        return PGC_ERR_BOUNDS;
+    if (batch == 0 || total_q == 0 || max_q_len == 0) return PGC_OK;
+    if (!q || !k_pages || !v_pages || !block_tables || !q_starts || !seq_lens || !out ||
+        (weights && !weights->weights) || max_pages_per_seq == 0 || max_seq_len == 0)
+        return PGC_ERR_INVALID;
+    if ((int64_t)max_pages_per_seq * PGC_PAGE_TOKENS < max_seq_len) return PGC_ERR_BOUNDS;
+    if (num_pages * 4 * 16 > INT32_MAX) return PGC_ERR_BOUNDS;  // TMA row coordinate is int32
+    if (total_q > PGC_CHUNK_MAX_ROWS || max_seq_len > PGC_CHUNK_MAX_TOKENS) return PGC_ERR_BOUNDS;
+    if (!al16(q) || !al16(k_pages) || !al16(v_pages) || !al16(gate) || !al16(out) || !al16(workspace) ||
+        ((uintptr_t)lse & 3u) != 0 || (weights && ((uintptr_t)weights->weights & 3u) != 0))
+        return PGC_ERR_ALIGN;
+    const int sms = current_sm_count();
+    if (!workspace || workspace_bytes < chunk_workspace_bytes(batch, total_q, max_q_len, max_seq_len,
+                                                              weights != nullptr, sms))
+        return PGC_ERR_WORKSPACE;
+    int st = check_device(nullptr);
+    if (st != PGC_OK) return st;
+    CUtensorMap tk, tv;
+    if ((st = pool_tensor_map(k_pages, num_pages, &tk)) != PGC_OK) return st;
+    if ((st = pool_tensor_map(v_pages, num_pages, &tv)) != PGC_OK) return st;
+    RaggedBatch rag;
+    rag.q_starts = q_starts;
+    rag.seq_lens = seq_lens;
+    rag.batch = batch;
+    rag.total_q = total_q;
+    rag.max_q_len = max_q_len;
+    rag.max_seq_len = max_seq_len;
+    return cuda_status(launch_chunk(q, tk, tv, k_pages, v_pages, num_pages, block_tables, max_pages_per_seq, rag,
+                                    scale, gate, out, lse, weights, workspace, sms,
+                                    static_cast<cudaStream_t>(stream)));
+}
+
+int pgc_chunk_attn(const uint16_t *q, const uint16_t *k_pages, const uint16_t *v_pages, int64_t num_pages,
+                   const int32_t *block_tables, int max_pages_per_seq, const int32_t *q_starts,
+                   const int32_t *seq_lens, int batch, int total_q, int max_q_len, int max_seq_len, float scale,
+                   const uint16_t *gate, uint16_t *out, float *lse, void *workspace, size_t workspace_bytes,
+                   void *stream) {
+    return chunk_call(q, k_pages, v_pages, num_pages, block_tables, max_pages_per_seq, q_starts, seq_lens, batch,
+                      total_q, max_q_len, max_seq_len, scale, gate, out, lse, nullptr, workspace, workspace_bytes,
+                      stream);
+}
+
+int pgc_chunk_attn_weights(const uint16_t *q, const uint16_t *k_pages, const uint16_t *v_pages, int64_t num_pages,
+                           const int32_t *block_tables, int max_pages_per_seq, const int32_t *q_starts,
+                           const int32_t *seq_lens, int batch, int total_q, int max_q_len, int max_seq_len,
+                           float scale, const uint16_t *gate, uint16_t *out, float *lse, float *weights,
+                           int64_t weights_stride, int64_t num_slots, const int32_t *slots, void *workspace,
+                           size_t workspace_bytes, void *stream) {
+    ChunkWeights w;
+    w.weights = weights;
+    w.stride = weights_stride;
+    w.num_slots = num_slots;
+    w.slots = slots;
+    return chunk_call(q, k_pages, v_pages, num_pages, block_tables, max_pages_per_seq, q_starts, seq_lens, batch,
+                      total_q, max_q_len, max_seq_len, scale, gate, out, lse, &w, workspace, workspace_bytes, stream);
+}
+
+int pgc_kv_evict_select(const float *weights, float *weights_out, int64_t weights_stride, int64_t num_slots,
+                        const int32_t *slots, const int32_t *seq_lens, int batch, int max_seq_len, int budget,
+                        int keep_first, int keep_last, int32_t *kept, int32_t *new_lens, void *stream) {
+    if (batch < 0 || max_seq_len < 0 || num_slots <= 0 || budget < 1 || keep_first < 0 || keep_last < 0 ||
+        (int64_t)keep_first + keep_last > budget)
+        return PGC_ERR_INVALID;
+    if (batch > 65535 || max_seq_len > PGC_EVICT_MAX_TOKENS || weights_stride < max_seq_len ||
+        (!slots && batch > num_slots))
+        return PGC_ERR_BOUNDS;
+    if (batch == 0) return PGC_OK;
+    if (!weights || !seq_lens || !kept || new_lens == seq_lens) return PGC_ERR_INVALID;
+    if (((uintptr_t)weights & 3u) != 0 || ((uintptr_t)weights_out & 3u) != 0) return PGC_ERR_ALIGN;
+    const int st = check_device(nullptr);
+    if (st != PGC_OK) return st;
+    return cuda_status(launch_evict_select(weights, weights_out, weights_stride, num_slots, slots, seq_lens, batch,
+                                           max_seq_len, budget, keep_first, keep_last, kept, new_lens,
+                                           static_cast<cudaStream_t>(stream)));
+}
+
+int pgc_kv_evict_compact(const uint16_t *src_k_pages, const uint16_t *src_v_pages, int64_t src_num_pages,
+                         const int32_t *src_tables, int src_max_pages, const int32_t *kept, int batch, int budget,
+                         uint16_t *dst_k_pages, uint16_t *dst_v_pages, int64_t dst_num_pages,
+                         const int32_t *dst_tables, int dst_max_pages, void *stream) {
+    if (batch < 0 || budget < 0 || src_num_pages <= 0 || dst_num_pages <= 0 || src_max_pages < 0 || dst_max_pages < 0)
+        return PGC_ERR_INVALID;
+    if (batch == 0 || budget == 0) return PGC_OK;
+    if (!src_k_pages || !src_v_pages || !src_tables || !kept || !dst_k_pages || !dst_v_pages || !dst_tables)
+        return PGC_ERR_INVALID;
+    if ((int64_t)dst_max_pages * PGC_PAGE_TOKENS < budget) return PGC_ERR_BOUNDS;
+    if ((int64_t)batch * budget > INT32_MAX / 4) return PGC_ERR_BOUNDS;  // rows, the grid
+    if (!al16(src_k_pages) || !al16(src_v_pages) || !al16(dst_k_pages) || !al16(dst_v_pages)) return PGC_ERR_ALIGN;
+    const int st = check_device(nullptr);
+    if (st != PGC_OK) return st;
+    return cuda_status(launch_evict_compact(src_k_pages, src_v_pages, src_num_pages, src_tables, src_max_pages, kept,
+                                            batch, budget, dst_k_pages, dst_v_pages, dst_num_pages, dst_tables,
+                                            dst_max_pages, static_cast<cudaStream_t>(stream)));
 }
 
 int pgc_copy_rows(void *dst, const void *src, const int32_t *dst_rows, const int32_t *src_rows,

@@ -42,6 +42,8 @@ enum ErrCode : int {
     kErrWaitTimeout = 4,
     kErrTableOutOfRange = 5,
     kErrSmemAlign = 6,
+    kErrRowsOutOfRange = 7,  // a ragged batch's query rows
+    kErrLenOutOfRange = 8,   // a sequence length above the host bound
 };
 
 #define PGC_DEFINE_ERROR_WORD(name) static __device__ pgc::DevError name

@@ -29,6 +29,18 @@ int q_tensor_map(const void *q, int tokens, CUtensorMap *out);
 int tiled_map_2d(const void *ptr, int elem_bytes, int64_t inner, int64_t outer, int box_inner,
                  int box_outer, bool swizzle128, CUtensorMap *out);
 
+// A ragged batch: sequence b's query rows are [q_starts[b], q_starts[b + 1]) of the q, gate, out
+// and lse arrays, and the last of them is the last token of its cache of seq_lens[b] tokens. The
+// device arrays are checked against the host bounds by every kernel that reads them.
+struct RaggedBatch {
+    const int32_t *q_starts = nullptr;  // [batch + 1]
+    const int32_t *seq_lens = nullptr;  // [batch]
+    int batch = 0;
+    int total_q = 0;
+    int max_q_len = 0;
+    int max_seq_len = 0;
+};
+
 // decode_attn.cu
 struct DecodePlan {
     int pages_per_split;
@@ -66,6 +78,13 @@ cudaError_t launch_merge_partials(const float *partials, int64_t rows, int num_p
                                   int64_t part_stride, const uint16_t *gate, uint16_t *out,
                                   cudaStream_t stream);
 cudaError_t decode_read_error(DevErrorHost *e, bool clear);
+// the split kernel over a ragged batch of at most PGC_MAX_QUERIES rows a sequence: partials
+// [total_q * 16][decode_plan().max_splits][258]; scores nullable
+cudaError_t launch_ragged_split(const uint16_t *q, const CUtensorMap &tk, const CUtensorMap &tv,
+                                int64_t num_pages, const int32_t *block_tables, int max_pages_per_seq,
+                                const RaggedBatch &rag, float scale, float *parts, float *scores,
+                                int64_t score_stride, const void *k_pages, const void *v_pages,
+                                int sm_count, cudaStream_t stream);
 // context-parallel exchange buffer: [2][world][16][8][34] u64 epoch-tagged words
 size_t cp_buffer_bytes(int world);
 cudaError_t launch_cp_decode(const uint16_t *q, const CUtensorMap &tk, const CUtensorMap &tv,
@@ -113,6 +132,38 @@ cudaError_t launch_prefill(const uint16_t *q, const CUtensorMap &tk, const CUten
                            int chunk_len, float scale, uint16_t *out, void *workspace,
                            int sm_count, cudaStream_t stream);
 cudaError_t prefill_read_error(DevErrorHost *e, bool clear);
+
+// chunk_attn.cu
+struct ChunkWeights {
+    float *weights;  // [num_slots][4][stride]
+    int64_t stride, num_slots;
+    const int32_t *slots;  // [batch], nullable
+};
+size_t chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count);
+cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtensorMap &tv, const uint16_t *k_pages,
+                         const uint16_t *v_pages, int64_t num_pages, const int32_t *block_tables,
+                         int max_pages_per_seq, const RaggedBatch &rag, float scale, const uint16_t *gate,
+                         uint16_t *out, float *lse, const ChunkWeights *weights, void *workspace, int sm_count,
+                         cudaStream_t stream);
+cudaError_t chunk_read_error(DevErrorHost *e, bool clear);
+
+// chunk_weights.cu: weights += column sums of exp(scale q.k - lse) over the batch's rows
+cudaError_t launch_chunk_weights(const CUtensorMap &tq, const CUtensorMap &tk, int64_t num_pages,
+                                 const int32_t *block_tables, int max_pages_per_seq, const RaggedBatch &rag,
+                                 float scale, const float *lse, const ChunkWeights &weights, int sm_count,
+                                 cudaStream_t stream);
+cudaError_t chunk_weights_read_error(DevErrorHost *e, bool clear);
+
+// kv_evict.cu
+cudaError_t launch_evict_select(const float *weights, float *weights_out, int64_t stride, int64_t num_slots,
+                                const int32_t *slots, const int32_t *seq_lens, int batch, int max_seq_len,
+                                int budget, int keep_first, int keep_last, int32_t *kept, int32_t *new_lens,
+                                cudaStream_t stream);
+cudaError_t launch_evict_compact(const uint16_t *k_src, const uint16_t *v_src, int64_t src_pages,
+                                 const int32_t *src_tables, int src_max_pages, const int32_t *kept, int batch,
+                                 int budget, uint16_t *k_dst, uint16_t *v_dst, int64_t dst_pages,
+                                 const int32_t *dst_tables, int dst_max_pages, cudaStream_t stream);
+cudaError_t evict_read_error(DevErrorHost *e, bool clear);
 
 // linear_attn.cu
 size_t gated_delta_prefill_workspace_bytes(int tokens);
