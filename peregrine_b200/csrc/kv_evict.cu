@@ -18,15 +18,20 @@ PGC_DEFINE_ERROR_WORD(g_evict_err);
 namespace {
 
 // ---------------------------------------------------------------- selection
-// A cluster of 1-8 CTAs per (sequence, kv head); each CTA keeps its consecutive share of the weights
-// in shared memory, so they are read from HBM once. The weight of rank B - F - R is found from the
-// top bits down: three histograms (11, 11 and 10 bits of the weight's bits in an order-preserving
-// form) of the candidates that share the bits found so far, summed over the cluster through
-// distributed shared memory. Then each warp counts its segment's kept tokens with ballots, the
-// counts are scanned over warps and CTAs, and the tokens are written in order.
-constexpr int kSelThreads = 512;
-constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kBins = 2048;
+// A cluster of 1-8 CTAs per (sequence, kv head). Each warp holds a segment of the row in registers, as
+// order-preserving integers: the first and last tokens as the greatest, places past the row's end as
+// the smallest, so that one rule serves all. The value of rank B is found from its top byte down: a
+// histogram of the next byte of the values that share the bytes found so far, summed over the cluster
+// through distributed shared memory, up to four times; it stops when all that share them are kept.
+// Then the warps count what they keep, the counts are scanned over warps and CTAs, and the tokens are
+// written in order.
+// The histogram has a column per lane: lane l adds to hist[byte][l], its own bank, so a warp's adds
+// never meet however the weights cluster (attention weights share a few exponents; with one shared
+// column those adds ran one after the other: 519 us for 64 sequences of up to 65536 tokens). What
+// bounds the kernel is the instructions issued, some 50 per 32 weights, and the cluster barriers.
+constexpr int kBins = 256;
+constexpr int kMaxPer = 32;  // weights a thread
+static_assert(8 * 1024 * kMaxPer >= PGC_EVICT_MAX_TOKENS, "the longest row does not fit a cluster");
 
 struct SelectParams {
     const float *weights;
@@ -40,11 +45,12 @@ struct SelectParams {
     int32_t *new_lens;
 };
 
-// Unsigned integers in the order of the floats, -0 and +0 alike, NaN below everything.
+// A weight as it is held and moved: -0 as +0, every NaN as the one whose order bits are 0.
+__device__ __forceinline__ float canonical(float x) { return x == x ? x + 0.f : __uint_as_float(0xffffffffu); }
+// Unsigned integers in the order of the canonical floats, NaN below everything.
 __device__ __forceinline__ uint32_t order_bits(float x) {
-    if (x != x) return 0;
-    const uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
-    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    const int32_t u = __float_as_int(x);
+    return (uint32_t)u ^ ((uint32_t)(u >> 31) | 0x80000000u);
 }
 
 __device__ __forceinline__ uint32_t ctas_in_cluster() {
@@ -68,18 +74,28 @@ __device__ __forceinline__ uint32_t load_peer(const void *p, uint32_t cta) {
     return v;
 }
 
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const SelectParams p) {
-    extern __shared__ float vals[];  // this CTA's share of the weights
-    __shared__ uint32_t hist[2][kBins];
-    __shared__ uint32_t warp_sum[kSelWarps];
-    __shared__ uint32_t found[2];                // the bin and the candidates above it
-    __shared__ uint32_t cnt[2];                  // this CTA's kept tokens apart from ties, and its ties
+template <int kSelThreads, int kPer>  // kPer: weights a thread, at most
+__global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_kernel(const SelectParams p) {
+    constexpr int kSelWarps = kSelThreads / 32;
+    extern __shared__ uint32_t dyn[];
+    uint32_t *hist = dyn;                                       // [256][32 lanes]
+    float *vals = reinterpret_cast<float *>(dyn + kBins * 32);  // this CTA's share of the weights
+    __shared__ uint32_t totals[2][kBins];  // this CTA's histogram, read by the cluster
+    __shared__ uint32_t warp_sum[kBins / 32];
+    __shared__ uint32_t found[3];  // the byte, the values above it and of it
+    __shared__ uint32_t cnt[2];    // values above the ties in this CTA, and ties
     __shared__ uint32_t seg_sure[kSelWarps], seg_tie[kSelWarps];
     pdl_trigger();
     pdl_wait();
     const uint32_t rank = cta_in_cluster(), ctas = ctas_in_cluster();
     const int h = blockIdx.y, b = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto sync_all = [&]() {
+        if (ctas > 1)
+            cluster_sync();
+        else
+            __syncthreads();
+    };
     const bool reporter = h == 0 && rank == 0;
     int32_t *kept = p.kept + ((int64_t)b * kNumKvHeads + h) * p.budget;
 
@@ -94,137 +110,171 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const SelectP
     const int n_new = min(L, B);
     if (reporter && tid == 0 && p.new_lens != nullptr) p.new_lens[b] = n_new;
     for (int i = n_new + (int)rank * kSelThreads + tid; i < B; i += (int)ctas * kSelThreads) kept[i] = -1;
-    const float *w = p.weights + (slot * kNumKvHeads + h) * p.stride;
-    float *wo = p.weights_out + (slot * kNumKvHeads + h) * p.stride;
+    const int64_t row = (max(slot, (int64_t)0) * kNumKvHeads + h) * p.stride;
+    const float *w = p.weights + row;
+    float *wo = p.weights_out != nullptr ? p.weights_out + row : nullptr;
     if (L <= B) {  // uniform over the cluster
         for (int i = (int)rank * kSelThreads + tid; i < L; i += (int)ctas * kSelThreads) {
             kept[i] = i;
-            if (p.weights_out != nullptr && p.weights_out != p.weights) wo[i] = w[i];
+            if (wo != nullptr && wo != w) wo[i] = w[i];
         }
         return;
     }
 
-    // shares of whole warp segments
-    const int seg = (int)(((int64_t)L + (int64_t)ctas * kSelThreads - 1) / ((int64_t)ctas * kSelThreads)) * 32;
-    const int share = seg * kSelWarps;
-    const int t0 = min(L, (int)rank * share), n = min(L, t0 + share) - t0;
-#pragma unroll 4
-    for (int i = tid; i < n; i += kSelThreads) vals[i] = w[t0 + i];
-    for (int i = tid; i < 2 * kBins; i += kSelThreads) (&hist[0][0])[i] = 0;
+    // warp segments of `per` x 32 consecutive weights; element j of a lane is number j * 32 + lane.
+    // `per` is a multiple of 4, so that the loops below test it once per 4 elements.
+    const int per = (int)(((int64_t)L + (int64_t)ctas * kSelThreads * 4 - 1) / ((int64_t)ctas * kSelThreads * 4)) * 4;
+    const int i0 = warp * per * 32 + lane;        // in the CTA's share
+    const int t0 = (int)rank * per * kSelThreads;  // the share's first token
+    const int last = L - p.keep_last;
+    uint32_t key[kPer];
+#define PGC_EACH_KEY \
+    _Pragma("unroll") for (int j4 = 0; j4 < kPer; j4 += 4) if (j4 < per) _Pragma("unroll") for (int j = j4; j < j4 + 4; ++j)
+    PGC_EACH_KEY {
+        const int t = t0 + i0 + j * 32;
+        key[j] = t < L ? __float_as_uint(w[t]) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kBins * 32 / kSelThreads; ++i) hist[i * kSelThreads + tid] = 0;
+    PGC_EACH_KEY {
+        const int t = t0 + i0 + j * 32;
+        const float x = canonical(__uint_as_float(key[j]));
+        if (wo != nullptr) vals[i0 + j * 32] = x;
+        key[j] = t >= L ? 0u : (t < p.keep_first || t >= last) ? 0xffffffffu : order_bits(x);
+    }
     __syncthreads();
 
-    const int lo = p.keep_first, hi = L - p.keep_last;  // candidates
-    uint32_t need = (uint32_t)(B - p.keep_first - p.keep_last);
-    uint32_t prefix = 0;  // bits found so far
-    if (need > 0) {
-        int known = 0;  // how many
+    // Values that begin with the bytes found lie in [tie_lo, tie_lo + tie_width]: the ties; those
+    // above are kept, and `need` of the ties, the first in order. Places past the row's end may tie
+    // with NaN weights only, which come before them.
+    const uint32_t hist_lane = smem_u32(hist) + lane * 4;
+    uint32_t need = (uint32_t)B, tie_lo = 0, tie_width = 0xffffffffu, ties = 0;
 #pragma unroll 1
-        for (int pass = 0; pass < 3; ++pass) {
-            const int bits = pass < 2 ? 11 : 10, shift = 32 - known - bits;
-            uint32_t *hh = hist[pass & 1];
-            for (int i = tid; i < n; i += kSelThreads) {
-                const int t = t0 + i;
-                const uint32_t k = order_bits(vals[i]);
-                if (t >= lo && t < hi && (pass == 0 || (k >> (32 - known)) == prefix))
-                    atomicAdd(&hh[(k >> shift) & ((1u << bits) - 1)], 1u);
-            }
-            cluster_sync();
-            // Sum over the cluster, bins from the top: thread i holds bins top - 4 i .. - 3.
-            uint32_t c[4], sum = 0;
+    for (int sh = 24; sh >= 0; sh -= 8) {
+        const uint32_t buf = (sh >> 3) & 1;
+        // predicated adds: a branch around each costs more than the add
+        PGC_EACH_KEY {
+            asm volatile(
+                "{\n\t.reg .pred in;\n\t"
+                "setp.le.u32 in, %0, %1;\n\t"
+                "@in red.shared.add.u32 [%2], 1;\n\t}"
+                ::"r"(key[j] - tie_lo), "r"(tie_width), "r"(hist_lane + ((key[j] >> sh) & 255u) * 128)
+                : "memory");
+        }
+        __syncthreads();
+        // warp w sums the columns of 8 bytes and clears them for the next round
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int bin = kBins - 1 - (tid * 4 + k);
-                c[k] = 0;
-                for (uint32_t q = 0; q < ctas; ++q) c[k] += q == rank ? hh[bin] : load_peer(&hh[bin], q);
-                sum += c[k];
+        for (int k = 0; k < kBins / kSelWarps; ++k) {
+            const int bin = warp * (kBins / kSelWarps) + k;
+            const uint32_t sum = __reduce_add_sync(0xffffffffu, hist[bin * 32 + lane]);
+            hist[bin * 32 + lane] = 0;
+            if (lane == 0) totals[buf][bin] = sum;
+        }
+        // also orders the clearing before the next round's adds; totals are double-buffered, so a
+        // peer's reads of a round are over when this CTA writes that buffer again
+        sync_all();
+        // thread i < 256: byte 255 - i over the cluster, then the sum of those above it
+        uint32_t c = 0, incl = 0;
+        const int bin = kBins - 1 - tid;
+        if (tid < kBins) {
+            if (ctas > 1) {
+                uint32_t v[8];
+#pragma unroll
+                for (uint32_t q = 0; q < 8; ++q) v[q] = q < ctas ? load_peer(&totals[buf][bin], q) : 0;
+#pragma unroll
+                for (uint32_t q = 0; q < 8; ++q) c += v[q];
+            } else {
+                c = totals[buf][bin];
             }
-            uint32_t incl = sum;
+            incl = c;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += v;
+                const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += x;
             }
             if (lane == 31) warp_sum[warp] = incl;
-            // the other buffer is cleared for the next pass: its last readers were the pass before
-            // this one's cluster barrier
-            for (int i = tid; i < kBins; i += kSelThreads) hist[(pass & 1) ^ 1][i] = 0;
-            __syncthreads();
-            uint32_t above = incl - sum;
-            for (int q = 0; q < warp; ++q) above += warp_sum[q];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (above < need && above + c[k] >= need) {
-                    found[0] = (uint32_t)(kBins - 1 - (tid * 4 + k));
-                    found[1] = above;
-                }
-                above += c[k];
-            }
-            __syncthreads();
-            prefix = (prefix << bits) | found[0];
-            need -= found[1];
-            known += bits;
         }
+        __syncthreads();
+        if (tid < kBins) {
+            uint32_t above = incl - c;
+            for (int q = 0; q < warp; ++q) above += warp_sum[q];
+            if (above < need && above + c >= need) {
+                found[0] = (uint32_t)bin;
+                found[1] = above;
+                found[2] = c;
+            }
+        }
+        __syncthreads();
+        need -= found[1];
+        ties = found[2];
+        tie_lo |= found[0] << sh;
+        tie_width = (1u << sh) - 1;
+        if (ties == need) break;  // uniform over the cluster
     }
-    // Kept: the first and last, candidates above `prefix`, and the first `need` equal to it.
-    const bool middle = B > p.keep_first + p.keep_last;
-    auto classify = [&](int i, bool &sure, bool &tie) {
-        const int t = t0 + i;
-        const bool in = i < n;
-        const uint32_t k = in ? order_bits(vals[i]) : 0;
-        const bool cand = in && t >= lo && t < hi;
-        sure = in && (t < lo || t >= hi || (middle && k > prefix));
-        tie = cand && middle && k == prefix;
-    };
+
     uint32_t n_sure = 0, n_tie = 0;
-    for (int s = 0; s < seg; s += 32) {
-        bool sure, tie;
-        classify(warp * seg + s + lane, sure, tie);
-        n_sure += __popc(__ballot_sync(0xffffffffu, sure));
-        n_tie += __popc(__ballot_sync(0xffffffffu, tie));
+    PGC_EACH_KEY {
+        n_tie += key[j] - tie_lo <= tie_width;
+        n_sure += key[j] > tie_lo + tie_width;
     }
+    n_sure = __reduce_add_sync(0xffffffffu, n_sure);
+    n_tie = __reduce_add_sync(0xffffffffu, n_tie);
     if (lane == 0) {
         seg_sure[warp] = n_sure;
         seg_tie[warp] = n_tie;
     }
     __syncthreads();
-    if (tid == 0) {
-        uint32_t s = 0, e = 0;
-        for (int q = 0; q < kSelWarps; ++q) {
-            s += seg_sure[q];
-            e += seg_tie[q];
+    const uint32_t ws = lane < kSelWarps ? seg_sure[lane] : 0, wt = lane < kSelWarps ? seg_tie[lane] : 0;
+    uint32_t sure_before = __reduce_add_sync(0xffffffffu, lane < warp ? ws : 0);
+    uint32_t tie_before = __reduce_add_sync(0xffffffffu, lane < warp ? wt : 0);
+    if (warp == 0) {
+        const uint32_t s = __reduce_add_sync(0xffffffffu, ws), e = __reduce_add_sync(0xffffffffu, wt);
+        if (lane == 0) {
+            cnt[0] = s;
+            cnt[1] = e;
         }
-        cnt[0] = s;
-        cnt[1] = e;
     }
-    cluster_sync();
-    uint32_t sure_before = 0, tie_before = 0;
-    for (uint32_t q = 0; q < rank; ++q) {
-        sure_before += load_peer(&cnt[0], q);
-        tie_before += load_peer(&cnt[1], q);
-    }
-    for (int q = 0; q < warp; ++q) {
-        sure_before += seg_sure[q];
-        tie_before += seg_tie[q];
+    // from here on every CTA has read its weights: writing in place is safe
+    sync_all();
+    {
+        const uint32_t s = lane < (int)rank ? load_peer(&cnt[0], lane) : 0;
+        const uint32_t e = lane < (int)rank ? load_peer(&cnt[1], lane) : 0;
+        sure_before += __reduce_add_sync(0xffffffffu, s);
+        tie_before += __reduce_add_sync(0xffffffffu, e);
     }
     const uint32_t lt = (1u << lane) - 1;
-    for (int s = 0; s < seg; s += 32) {
-        const int i = warp * seg + s + lane;
-        bool sure, tie;
-        classify(i, sure, tie);
-        const uint32_t ms = __ballot_sync(0xffffffffu, sure), mt = __ballot_sync(0xffffffffu, tie);
-        const uint32_t rank_t = tie_before + __popc(mt & lt);
-        if (sure || (tie && rank_t < need)) {
-            const uint32_t at = sure_before + __popc(ms & lt) + min(rank_t, need);
-            kept[at] = t0 + i;
-            if (p.weights_out != nullptr) wo[at] = vals[i];
+    const bool all_ties = ties == need;
+    if (all_ties) {
+        // everything from tie_lo on is kept
+        uint32_t at = sure_before + tie_before;
+        PGC_EACH_KEY {
+            const bool keep = key[j] >= tie_lo;
+            const uint32_t m = __ballot_sync(0xffffffffu, keep);
+            if (keep) {
+                const uint32_t o = at + __popc(m & lt);
+                kept[o] = t0 + i0 + j * 32;
+                if (wo != nullptr) wo[o] = vals[i0 + j * 32];
+            }
+            at += __popc(m);
         }
-        sure_before += __popc(ms);
-        tie_before += __popc(mt);
+    } else {
+        PGC_EACH_KEY {
+            const bool sure = key[j] > tie_lo + tie_width, tie = key[j] - tie_lo <= tie_width;
+            const uint32_t ms = __ballot_sync(0xffffffffu, sure), mt = __ballot_sync(0xffffffffu, tie);
+            const uint32_t rank_t = tie_before + __popc(mt & lt);
+            if (sure || (tie && rank_t < need)) {
+                const uint32_t o = sure_before + __popc(ms & lt) + min(rank_t, need);
+                kept[o] = t0 + i0 + j * 32;
+                if (wo != nullptr) wo[o] = vals[i0 + j * 32];
+            }
+            sure_before += __popc(ms);
+            tie_before += __popc(mt);
+        }
     }
-    // every CTA has read its share (the cluster barriers above), so in place is safe
-    if (p.weights_out != nullptr)
+#undef PGC_EACH_KEY
+    if (wo != nullptr)
         for (int i = B + (int)rank * kSelThreads + tid; i < L; i += (int)ctas * kSelThreads) wo[i] = 0.f;
-    cluster_sync();  // a peer may still read this CTA's counts
+    if (ctas > 1) cluster_sync();  // a peer may still read this CTA's counts
 }
 
 // ---------------------------------------------------------------- compaction
@@ -316,24 +366,42 @@ cudaError_t launch_evict_select(const float *weights, float *weights_out, int64_
     p.keep_last = keep_last;
     p.kept = kept;
     p.new_lens = new_lens;
-    // CTAs per row: enough that a CTA's share is at most 8192 weights
-    int ctas = 1;
-    while (ctas < 8 && max_seq_len > ctas * 8192) ctas *= 2;
-    // the largest share: whole warp segments of ceil(L / (ctas * threads)) x 32
-    const int64_t per = ((int64_t)max_seq_len + (int64_t)ctas * kSelThreads - 1) / ((int64_t)ctas * kSelThreads);
-    const size_t smem = (size_t)per * kSelThreads * sizeof(float);
-    static std::atomic<bool> attr_set[64] = {};
-    int dev = 0;
+    // Threads and CTAs per row: at least what keeps a thread within kMaxPer weights, 512 threads while
+    // they suffice (two CTAs an SM overlap their barriers and loads); a batch that leaves SMs free
+    // takes more CTAs, up to 8, down to kSplitPer weights a thread, below which the cluster's barriers
+    // cost more than they save.
+    constexpr int kSplitPer = 8;
+    int sms = 148, dev = 0;
     cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int threads = max_seq_len > 8 * 512 * kMaxPer ? 1024 : 512;
+    auto weights_per_thread = [&](int c) { return (int)(((int64_t)max_seq_len + (int64_t)c * threads - 1) / ((int64_t)c * threads)); };
+    int ctas = 1;
+    while (ctas < 8 && (weights_per_thread(ctas) > kMaxPer ||
+                        ((int64_t)batch * kNumKvHeads * ctas * 2 <= sms && weights_per_thread(ctas) > kSplitPer)))
+        ctas *= 2;
+    const int per = weights_per_thread(ctas);
+    struct Variant {
+        void (*kern)(const SelectParams);
+        int threads, per;
+    };
+    const Variant variants[] = {{evict_select_kernel<512, 8>, 512, 8}, {evict_select_kernel<512, 16>, 512, 16},
+                                {evict_select_kernel<512, 32>, 512, 32}, {evict_select_kernel<1024, 32>, 1024, 32}};
+    const size_t hist_bytes = kBins * 32 * sizeof(uint32_t);
+    static std::atomic<bool> attr_set[64] = {};
     if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             PGC_EVICT_MAX_TOKENS / 8 * (int)sizeof(float));
-        if (e != cudaSuccess) return e;
+        for (const Variant &v : variants) {
+            cudaError_t e = cudaFuncSetAttribute(v.kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)(hist_bytes + v.threads * v.per * sizeof(float)));
+            if (e != cudaSuccess) return e;
+        }
         if (dev >= 0 && dev < 64) attr_set[dev] = true;
     }
+    const auto kern = threads == 1024 ? variants[3].kern : variants[per <= 8 ? 0 : per <= 16 ? 1 : 2].kern;
+    const size_t smem = hist_bytes + (weights_out != nullptr ? (size_t)(per + 3) / 4 * 4 * threads * sizeof(float) : 0);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, kNumKvHeads, batch);
-    cfg.blockDim = dim3(kSelThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -349,7 +417,7 @@ cudaError_t launch_evict_select(const float *weights, float *weights_out, int64_
 #else
     cfg.numAttrs = 1;
 #endif
-    return cudaLaunchKernelEx(&cfg, evict_select_kernel, p);
+    return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
 cudaError_t launch_evict_compact(const uint16_t *k_src, const uint16_t *v_src, int64_t src_pages,
