@@ -245,12 +245,12 @@ int pgc_prefill_attn(const uint16_t *q, const uint16_t *k_pages, const uint16_t 
  * ------------------------------------------------------------------------------------- */
 
 #define PGC_CHUNK_MAX_BATCH 4096
-#define PGC_CHUNK_MAX_ROWS (1 << 24)   /* query rows of a call */
+#define PGC_CHUNK_MAX_ROWS (1 << 22)   /* query rows of a call */
 #define PGC_CHUNK_MAX_TOKENS (1 << 24) /* tokens of a sequence */
 
 /* Workspace bytes of pgc_chunk_attn (with_weights = 0) and pgc_chunk_attn_weights (1). Up to
  * PGC_MAX_QUERIES rows a sequence: the splits' partials, and with weights 16 fp32 scores per query
- * row and token of max_seq_len. More rows: 37 MiB, and with weights the rows' lse. 0 for shapes that
+ * row and token of max_seq_len; more rows: 38 MiB; with weights the rows' lse too. 0 for shapes that
  * the entries refuse. */
 size_t pgc_chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_seq_len,
                                  int with_weights);

@@ -8,11 +8,14 @@
 // exp(s_t - lse). A row that sees nothing (p < 0) has o = 0 and lse = -inf.
 //
 // Two forms, chosen by the host bound on the rows of a sequence:
-//   * up to PGC_MAX_QUERIES rows: the split decode kernel over the ragged batch (decode_attn.cu),
-//     bound by the K/V bytes, then chunk_finish_kernel, which merges the splits and adds the
-//     weights from the scores that the split kernel left (one pass over K);
-//   * more rows: chunk_pair_kernel on the 5th-gen tensor cores, then chunk_merge_kernel for the
-//     rows whose key range was shared out, and chunk_weights.cu for the weights.
+//   * up to PGC_MAX_QUERIES rows: chunk_split_kernel (mma.sync), bound by the K/V bytes; with weights
+//     it leaves the scores in the workspace and chunk_add_kernel turns them into weights, so K is
+//     read once;
+//   * more rows: chunk_pair_kernel on the 5th-gen tensor cores, and chunk_weights.cu for the weights.
+// In both, the line of all the batch's tiles is cut into equal consecutive shares, one per CTA (or
+// pair) of a fixed grid: lengths are on the device, and the balance is within one tile whatever they
+// are. A unit of work cut by a share's border leaves fp32 partials, at most two units a share (its
+// first and its last), which the merge kernel joins; every other unit is written where it is computed.
 #include <cuda.h>
 
 #include "pgc_common.cuh"
@@ -31,222 +34,34 @@ __device__ __forceinline__ float sigmoid_gate(float v, uint32_t gate_bits) {
 }
 
 // =============================================================================================
-// Up to 4 rows a sequence: merge of the splits and the weights, one launch. Blocks [0, merge_blocks)
-// merge (one per row, head and 32-dim chunk; the 8 warps take every 8th split, as the uniform
-// batch's merge does); the rest add the weights of 1024 tokens of one (sequence, kv head) each,
-// from the scores in the workspace and the rows' lse, which they form from the splits' (m, l)
-// themselves: both halves start as soon as the split kernel has finished.
+// The schedule. A unit is a (sequence, kv head, block of kTok query tokens); its tiles are blocks of
+// kKeys keys. The line of work is the units' tiles, units in that order.
 // =============================================================================================
-struct FinishParams {
-    RaggedBatch rag;
-    const float *parts;  // [total_q * 16][max_splits][258]
-    int max_splits;
-    int merge_blocks;
-    const uint16_t *gate;
-    uint16_t *out;
-    float *lse;
-    // weights
-    const float *scores;  // [total_q][4][score_stride][4], scaled by log2(e)
-    int64_t score_stride;
-    float *weights;
-    int64_t weights_stride, num_slots;
-    const int32_t *slots;
-    int add_chunks;  // blocks per (sequence, kv head)
+struct PairTiling {
+    static constexpr int kTok = 64, kKeys = 128;
+    // A share below this many tiles costs more in its Q load, pipeline fill and partials than it saves.
+    static constexpr int kMinShare = 4;
+};
+struct SplitTiling {
+    static constexpr int kTok = PGC_MAX_QUERIES, kKeys = kPage;
+    static constexpr int kMinShare = 4;
 };
 
-constexpr int kFinishThreads = 256;
-constexpr int kAddTokens = 1024;
-
-__device__ __forceinline__ void finish_merge(const FinishParams &p, int blk) {
-    __shared__ float red_m[8], red_den[8], red_acc[8][32];
-    const int chunk = blk & 7;
-    const int head = (blk >> 3) & 15;
-    const int j = (blk >> 7) % p.rag.max_q_len;
-    const int b = (blk >> 7) / p.rag.max_q_len;
-    const RaggedSeq sv = ragged_seq(p.rag, b, nullptr);
-    if (j >= sv.n) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t row = (int64_t)(sv.row0 + j) * kNumQHeads + head;
-    const int d = chunk * 32 + lane;
-    const float *base = p.parts + row * p.max_splits * kPartial;
-    // 10 splits per warp are held in registers (one round of loads); longer rows stream them
-    constexpr int kCached = 10;
-    float ma = -INFINITY, den = 0.f, acc = 0.f;
-    float mc[kCached], lc[kCached], oc[kCached];
-#pragma unroll
-    for (int i = 0; i < kCached; ++i) {
-        const int c = warp + 8 * i;
-        mc[i] = -INFINITY;
-        lc[i] = oc[i] = 0.f;
-        if (c < p.max_splits) {
-            const float *pc = base + (int64_t)c * kPartial;
-            mc[i] = pc[0];
-            lc[i] = pc[1];
-            oc[i] = pc[2 + d];  // read even for an empty part: it is not summed
-        }
-        ma = fmaxf(ma, mc[i]);
-    }
-    for (int c = warp + 8 * kCached; c < p.max_splits; c += 8) ma = fmaxf(ma, base[(int64_t)c * kPartial]);
-    if (lane == 0) red_m[warp] = ma;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) ma = fmaxf(ma, red_m[w]);
-#pragma unroll
-    for (int i = 0; i < kCached; ++i) {
-        if (mc[i] == -INFINITY) continue;
-        const float w = exp2f((mc[i] - ma) * kLog2e);
-        den += lc[i] * w;
-        acc += oc[i] * w;
-    }
-    for (int c = warp + 8 * kCached; c < p.max_splits; c += 8) {
-        const float *pc = base + (int64_t)c * kPartial;
-        const float m = pc[0];
-        if (m == -INFINITY) continue;
-        const float w = exp2f((m - ma) * kLog2e);
-        den += pc[1] * w;
-        acc += pc[2 + d] * w;
-    }
-    red_acc[warp][lane] = acc;
-    if (lane == 0) red_den[warp] = den;
-    __syncthreads();
-    if (warp != 0) return;
-    acc = den = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-        acc += red_acc[w][lane];
-        den += red_den[w];
-    }
-    float v = (den == 0.f) ? 0.f : acc / den;
-    if (p.gate != nullptr) v = sigmoid_gate(v, p.gate[row * kHeadDim + d]);
-    p.out[row * kHeadDim + d] = f32_to_bf16_bits(v);
-    if (p.lse != nullptr && chunk == 0 && lane == 0) p.lse[row] = (den == 0.f) ? -INFINITY : ma + logf(den);
-}
-
-__device__ __forceinline__ void finish_add(const FinishParams &p, int blk) {
-    __shared__ float lse2[PGC_MAX_QUERIES * kGroup];
-    const int chunk = blk % p.add_chunks;
-    const int kvh = (blk / p.add_chunks) % kNumKvHeads;
-    const int b = blk / p.add_chunks / kNumKvHeads;
-    const RaggedSeq sv = ragged_seq(p.rag, b, nullptr);
-    const int t0 = chunk * kAddTokens;
-    if (sv.n == 0 || t0 >= sv.len) return;
-    const int64_t slot = ragged_slot(p.slots, p.num_slots, b, chunk == 0 && kvh == 0 ? &g_chunk_err : nullptr);
-    if (slot < 0) return;
-    // 16 threads per row: log2 of the row's sum over all splits; +inf where it is 0, so that a
-    // row of -inf scores adds nothing
-    {
-        const int r = threadIdx.x >> 4, part = threadIdx.x & 15;
-        const int np = r < sv.n * kGroup ? p.max_splits : 0;
-        const int64_t row = (int64_t)(sv.row0 + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup;
-        const float *base = p.parts + row * p.max_splits * kPartial;
-        float m = -INFINITY, l = 0.f;
-        for (int c = part; c < np; c += 16) m = fmaxf(m, base[(int64_t)c * kPartial]);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        for (int c = part; c < np; c += 16) {
-            const float mc = base[(int64_t)c * kPartial];
-            if (mc != -INFINITY) l += base[(int64_t)c * kPartial + 1] * exp2f((mc - m) * kLog2e);
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (part == 0) lse2[r] = l == 0.f ? INFINITY : m * kLog2e + log2f(l);
-    }
-    __syncthreads();
-    float *w = p.weights + (slot * kNumKvHeads + kvh) * p.weights_stride;
-    const float4 *s = reinterpret_cast<const float4 *>(p.scores);
-#pragma unroll
-    for (int i = 0; i < kAddTokens / kFinishThreads; ++i) {
-        const int t = t0 + i * kFinishThreads + threadIdx.x;
-        if (t >= sv.len) break;
-        float add = 0.f;
-        for (int j = 0; j < sv.n; ++j) {
-            if (t > sv.len - sv.n + j) continue;  // not visible to row j
-            const float4 x = s[((int64_t)(sv.row0 + j) * kNumKvHeads + kvh) * p.score_stride + t];
-            add += exp2f(x.x - lse2[j * kGroup]);
-            add += exp2f(x.y - lse2[j * kGroup + 1]);
-            add += exp2f(x.z - lse2[j * kGroup + 2]);
-            add += exp2f(x.w - lse2[j * kGroup + 3]);
-        }
-        w[t] += add;
-    }
-}
-
-__global__ void __launch_bounds__(kFinishThreads) chunk_finish_kernel(const FinishParams p) {
-    pdl_trigger();
-    pdl_wait();
-    if ((int)blockIdx.x < p.merge_blocks)
-        finish_merge(p, blockIdx.x);
-    else
-        finish_add(p, blockIdx.x - p.merge_blocks);
-}
-
-// =============================================================================================
-// More rows a sequence: two-SM tcgen05 kernel (cta_group::2). The tile of work and the roles are
-// those of the single-sequence prefill kernel: a cluster of two CTAs runs one kv head for 64 query
-// tokens (each CTA's 32 tokens x 4 GQA heads stacked into 128 rows, M = 256), each CTA stages its
-// own Q, 64 of a 128-key tile's keys and 128 of its value dims, S (two tiles) and O live in TMEM and
-// P is written over S. What differs is the schedule. Lengths are on the device, so the launch is a
-// fixed grid of one pair per two SMs, and the pairs share out the batch's key tiles: the tiles of
-// all (sequence, kv head, 64-token tile) units, in that order, form one line, which is cut into
-// equal consecutive shares. A unit cut by a share's border leaves fp32 partials (at most two units a
-// pair: its first and its last), which chunk_merge_kernel joins; every other unit is written by its
-// pair. The balance is then within one key tile whatever the lengths, and the workspace is fixed.
-// Loads, MMAs and softmax run on across units: the next unit's K, V and Q loads and its first S
-// products overlap this unit's last products and its epilogue.
-// =============================================================================================
-constexpr int kBM = 128;  // rows of a CTA: 32 tokens x 4 heads
-constexpr int kTokTile = 32;
-constexpr int kUnitTok = 2 * kTokTile;
-constexpr uint32_t kTmemCols = 512;
-constexpr float kLazyRescale = 8.0f;  // log2 units: rescale O only when the max grows by > 2^8
-constexpr int kSoftmaxWarps = 16;
-constexpr int kProducerWarps = 2;
-constexpr int kPairThreads = 32 * (kSoftmaxWarps + 1 + 2 * kProducerWarps);
-constexpr int kKeys = 128;                    // keys per tile
-constexpr int kQBytes = kBM * kHeadDim * 2;   // [4 dim blocks][128 rows][128 B]
-constexpr int kKHalf = 64 * kHeadDim * 2;     // this CTA's 64 keys: [4][64][128 B]
-constexpr int kVHalf = kKeys * 128 * 2;       // this CTA's 128 dims: [2][128][128 B]
-constexpr int kKSlots = 3;
-constexpr int kVSlots = 2;
-constexpr uint32_t kTO = 0;    // O: 256 columns
-constexpr uint32_t kTS = 256;  // S tiles: 2 x 128 columns; P(j) over the first 64 of S(j)
-// A share below this many tiles costs more in its Q load, pipeline fill and partials than it saves.
-constexpr int kMinShare = 4;
-
-// A fragment left in the workspace: rows [256][258] fp32 of one unit's tiles [t0, t1) of `tiles`.
-struct Fragment {
-    int seq;  // -1: none
-    int kvh, qt, last;  // last: it holds the unit's last tile
-};
-
-struct PairParams {
-    RaggedBatch rag;
-    const int32_t *block_tables;
-    int max_pages_per_seq;
-    int64_t num_pages;
-    const uint16_t *v_pages;
-    const uint16_t *gate;
-    uint16_t *out;
-    float *lse;
-    Fragment *frags;  // [pairs][2]: a share's first unit if cut before its first tile, its last if cut after
-    float *parts;     // [pairs][2][256][258]
-    float scale_log2;
-};
-
-// Key tiles of one unit: the keys that its last row sees, at least one tile (rows that see nothing
-// still get their zeros).
+// Tiles of one unit: the keys that its last row sees, at least one tile (rows that see nothing still
+// get their zeros).
+template <class T>
 __device__ __forceinline__ int unit_tiles(int n, int len, int qt) {
-    const int keys = len - n + min((qt + 1) * kUnitTok, n);
-    return keys > kKeys ? (keys + kKeys - 1) / kKeys : 1;
+    const int keys = len - n + min((qt + 1) * T::kTok, n);
+    return keys > T::kKeys ? (keys + T::kKeys - 1) / T::kKeys : 1;
 }
 
-// A pair's share as a walk over (unit, tile range); every role steps its own copy.
+// A share as a walk over (unit, tile range); every role steps its own copy.
 struct Walk {
     int seq, kvh, qt;
     int row0, n, len;  // of the sequence
     int tiles;         // of the unit
-    int t0, t1;        // this pair's tiles of it
-    int64_t left;      // tiles of the share from t0 on
+    int t0, t1;        // the share's tiles of it
+    int left;          // tiles of the share from t0 on
 };
 
 __device__ __forceinline__ void walk_seq(const RaggedBatch &rag, Walk &w) {
@@ -255,16 +70,18 @@ __device__ __forceinline__ void walk_seq(const RaggedBatch &rag, Walk &w) {
     w.n = s.n;
     w.len = s.len;
 }
+template <class T>
 __device__ __forceinline__ void walk_unit(Walk &w, int t0) {
-    w.tiles = unit_tiles(w.n, w.len, w.qt);
+    w.tiles = unit_tiles<T>(w.n, w.len, w.qt);
     w.t0 = t0;
-    w.t1 = (int64_t)w.tiles - t0 < w.left ? w.tiles : t0 + (int)w.left;
+    w.t1 = w.tiles - t0 < w.left ? w.tiles : t0 + w.left;
 }
 // Next unit; false at the end of the share.
+template <class T>
 __device__ __forceinline__ bool walk_next(const RaggedBatch &rag, Walk &w) {
     w.left -= w.t1 - w.t0;
     if (w.left <= 0) return false;
-    if (++w.qt * kUnitTok >= w.n) {
+    if (++w.qt * T::kTok >= w.n) {
         w.qt = 0;
         if (++w.kvh == kNumKvHeads) {
             w.kvh = 0;
@@ -274,37 +91,26 @@ __device__ __forceinline__ bool walk_next(const RaggedBatch &rag, Walk &w) {
             } while (w.n == 0);
         }
     }
-    walk_unit(w, 0);
+    walk_unit<T>(w, 0);
     return true;
 }
 
-struct PairSmem {
-    static constexpr int kQ = 0;
-    static constexpr int kK = kQ + kQBytes;
-    static constexpr int kV = kK + kKSlots * kKHalf;
-    static constexpr int kBar = kV + kVSlots * kVHalf;
-    // leader-side: q_full, k_full[3], v_full[2], p_full[2], o_free; both sides: q_empty, k_empty[3],
-    // v_empty[2], s_full[2], pv_done[2]
-    static constexpr int kNumBars = 2 + kKSlots + kVSlots + 2 + 1 + kKSlots + kVSlots + 2 + 2;
-    static constexpr int kRed = kBar + kNumBars * 8;
-    static constexpr int kWalk = kRed + 4 * kBM * 4;  // red: [4 key quarters][128 rows] fp32
-    static constexpr int kTmemSlot = kWalk + 48;
-    static constexpr int kAbort = kTmemSlot + 8;
-    static constexpr int kBytes = kAbort + 8;
+// The line's length and the shares it is cut into: share p is tiles [total * p / shares, total *
+// (p + 1) / shares).
+struct Line {
+    int64_t total;
+    int shares;
 };
-static_assert(sizeof(Walk) <= 48 && PairSmem::kWalk % 8 == 0, "walk slot");
-static_assert(PairSmem::kBytes <= 232448, "pair shared memory exceeds the sm_100 limit");
-static_assert(PGC_CHUNK_MAX_BATCH * 8 <= kKSlots * kKHalf, "the schedule's scratch is the K ring");
 
-// The share of pair `pair` of `pairs`: tiles [total * p / W, total * (p + 1) / W) of the line, over
-// W = min(pairs, total / kMinShare) pairs. Run by the whole CTA; `cost` is scratch (one int64 per
-// sequence). Returns false when the pair has no share.
-__device__ __forceinline__ bool find_share(const RaggedBatch &rag, int64_t *cost, int pair, int pairs, Walk *out,
-                                           DevError *err) {
+// Share `index` of a grid of `grid`, which uses min(grid, total / kMinShare) of them. Run by the whole
+// CTA; `cost` is scratch (one int64 per sequence). Returns false when the share is empty.
+template <class T>
+__device__ __forceinline__ bool find_share(const RaggedBatch &rag, int64_t *cost, int index, int grid, Walk *out,
+                                           Line *line, DevError *err) {
     for (int b = threadIdx.x; b < rag.batch; b += blockDim.x) {
         const RaggedSeq s = ragged_seq(rag, b, err);
         int64_t c = 0;
-        for (int qt = 0; qt * kUnitTok < s.n; ++qt) c += unit_tiles(s.n, s.len, qt);
+        for (int qt = 0; qt * T::kTok < s.n; ++qt) c += unit_tiles<T>(s.n, s.len, qt);
         cost[b] = c * kNumKvHeads;
     }
     __syncthreads();
@@ -314,12 +120,12 @@ __device__ __forceinline__ bool find_share(const RaggedBatch &rag, int64_t *cost
         for (int b = lane; b < rag.batch; b += 32) total += cost[b];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        int64_t w = total / kMinShare;
-        w = w < 1 ? 1 : w > pairs ? pairs : w;
-        const int64_t begin = total * pair / w, end = total * (pair + 1) / w;
+        int64_t w = total / T::kMinShare;
+        w = w < 1 ? 1 : w > grid ? grid : w;
+        const int64_t begin = total * index / w, end = total * (index + 1) / w;
         Walk wk = {};
         wk.seq = -1;
-        if (pair < w && end > begin) {
+        if (index < w && end > begin) {
             int64_t before = 0;
             for (int b0 = 0; b0 < rag.batch; b0 += 32) {
                 const int64_t c = b0 + lane < rag.batch ? cost[b0 + lane] : 0;
@@ -344,18 +150,528 @@ __device__ __forceinline__ bool find_share(const RaggedBatch &rag, int64_t *cost
             wk.kvh = (int)(off / per);
             off -= wk.kvh * per;
             for (wk.qt = 0;; ++wk.qt) {
-                const int t = unit_tiles(wk.n, wk.len, wk.qt);
+                const int t = unit_tiles<T>(wk.n, wk.len, wk.qt);
                 if (off < t) break;
                 off -= t;
             }
-            wk.left = end - begin;
-            walk_unit(wk, (int)off);
+            wk.left = (int)(end - begin);  // a grid of shares keeps it within int (PGC_CHUNK_MAX_ROWS)
+            walk_unit<T>(wk, (int)off);
         }
-        if (lane == 0) *out = wk;
+        if (lane == 0) {
+            *out = wk;
+            line->total = total;
+            line->shares = (int)w;
+        }
     }
     __syncthreads();
     return out->seq >= 0;
 }
+
+// A cut unit's record: slot 0 of a share is the unit that its start cuts, slot 1 the one that its end
+// cuts. Slot 1 names the share that ends the unit; the shares between hold its middle in their slot 0.
+struct Fragment {
+    int seq;  // -1: none
+    int kvh, qt;
+    int last;  // slot 1: the share with the unit's last tile
+};
+// `at`: the unit's tiles behind the share, which ends at total * (index + 1) / shares.
+__device__ __forceinline__ int share_of_end(const Line &line, int index, int64_t behind) {
+    const int64_t x = line.total * (index + 1) / line.shares + behind - 1;  // the unit's last tile
+    return (int)(((x + 1) * line.shares - 1) / line.total);
+}
+
+// =============================================================================================
+// Up to 4 rows a sequence. One CTA per share of 16-token pages: a producer warp streams each page's K
+// and V (8 KiB each) through a 4-stage ring by TMA, and consumer warp w takes every fourth page, with
+// the 4 GQA heads x up to 4 rows as the M = 16 of mma.m16n8k16, the online softmax in registers. The
+// tensor pipe is mostly idle (a kv head has 4 to 16 query rows): HBM bounds it. The producer and the
+// ring run on from unit to unit, Q is double-buffered, so only the end of the share drains.
+// Two CTAs an SM (register-bound) keep 128 KiB of pages in flight.
+// =============================================================================================
+constexpr int kConsumers = 4;
+constexpr int kSplitThreads = (kConsumers + 1) * 32;
+constexpr int kStages = 4;
+static_assert(kStages % kConsumers == 0, "each stage must belong to one consumer warp");
+constexpr int kTileBytes = kPage * kHeadDim * 2;  // one (page, kv head) of K or V: 8 KiB
+constexpr int kStageBytes = 2 * kTileBytes;
+constexpr int kRows = PGC_MAX_QUERIES * kGroup;
+constexpr int kQRowBytes = kHeadDim * 2 + 16;  // padded row: conflict-free ldmatrix
+constexpr int kJoinFloats = 4096;              // the warps' states are joined 16 KiB at a time
+
+struct SplitParams {
+    RaggedBatch rag;
+    const uint16_t *q;
+    const int32_t *block_tables;
+    int max_pages_per_seq;
+    int64_t num_pages;
+    const uint16_t *gate;
+    uint16_t *out;
+    float *lse;        // nullable
+    Fragment *frags;   // [shares][2]
+    float *parts;      // [shares][2][4 * max_q_len][258]
+    float *scores;     // nullable: [total_q][4][score_stride][4], scaled by log2(e)
+    int64_t score_stride;
+    float scale_log2;
+};
+
+struct SplitSmem {
+    static constexpr int kRing = 0;  // 1024-aligned
+    static constexpr int kQ = kRing + kStages * kStageBytes;
+    static constexpr int kJoin = kQ + 2 * kRows * kQRowBytes;
+    static constexpr int kM = kJoin + kJoinFloats * 4;  // [4 warps][16 rows]
+    static constexpr int kL = kM + kConsumers * kRows * 4;
+    static constexpr int kBar = kL + kConsumers * kRows * 4;  // full[4], empty[4], q_full[2], q_empty[2]
+    static constexpr int kWalk = kBar + (2 * kStages + 4) * 8;
+    static constexpr int kLine = kWalk + 48;
+    static constexpr int kBytes = kLine + 16;
+};
+constexpr int kSplitSmem = SplitSmem::kBytes + 1024;  // + alignment slack
+static_assert(sizeof(Walk) <= 48 && sizeof(Line) <= 16, "schedule slots");
+static_assert(PGC_CHUNK_MAX_BATCH * 8 <= kStages * kStageBytes, "the schedule's scratch is the ring");
+
+// Untiled bulk copy global -> shared, completion bytes on `bar`; 16-byte aligned, a multiple of 16.
+__device__ __forceinline__ void bulk_load(void *smem_dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(smem_dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+template <bool kScores>
+__global__ void __launch_bounds__(kSplitThreads, 2)
+    chunk_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                       const SplitParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + SplitSmem::kBar);
+    uint64_t *empty = full + kStages;
+    uint64_t *q_full = empty + kStages;
+    uint64_t *q_empty = q_full + 2;
+    Walk *share = reinterpret_cast<Walk *>(smem + SplitSmem::kWalk);
+    Line *line = reinterpret_cast<Line *>(smem + SplitSmem::kLine);
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int index = blockIdx.x;
+
+    pdl_trigger();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&q_full[s], 1);
+            mbar_init(&q_empty[s], kConsumers);
+        }
+        fence_mbar_init();
+        tma_prefetch_desc(&tmk);
+        tma_prefetch_desc(&tmv);
+    }
+    pdl_wait();
+    Fragment *frag = p.frags + index * 2;
+    if (threadIdx.x < 2) frag[threadIdx.x].seq = -1;
+    const bool busy = find_share<SplitTiling>(p.rag, reinterpret_cast<int64_t *>(smem + SplitSmem::kRing), index,
+                                              gridDim.x, share, line, index == 0 ? &g_chunk_err : nullptr);
+    if (!busy) return;
+    fence_proxy_async_smem();  // the schedule's scratch becomes the ring
+    __syncthreads();
+    Walk w = *share;
+
+    if (warp == kConsumers) {
+        // ------------------------------------------------------------ producer
+        const uint64_t pol = l2_policy_evict_first();
+        int g = 0;
+        for (int unit = 0;; ++unit) {
+            const int qb = unit & 1;
+            bool ok = true;
+            if (lane == 0) {
+                ok = unit < 2 || mbar_wait_bounded(&q_empty[qb], ((unit >> 1) - 1) & 1);
+                if (ok) {
+                    mbar_arrive_expect_tx(&q_full[qb], (uint32_t)w.n * kGroup * kHeadDim * 2);
+                    for (int r = 0; r < w.n * kGroup; ++r)
+                        bulk_load(smem + SplitSmem::kQ + (qb * kRows + r) * kQRowBytes,
+                                  p.q + ((int64_t)(w.row0 + r / kGroup) * kNumQHeads + w.kvh * kGroup + r % kGroup) * kHeadDim,
+                                  kHeadDim * 2, &q_full[qb]);
+                } else {
+                    record_error(&g_chunk_err, kErrWaitTimeout, 21);
+                }
+            }
+            const int32_t *table = p.block_tables + (int64_t)w.seq * p.max_pages_per_seq;
+            int ids = 0;
+            for (int t = w.t0; ok && t < w.t1; ++t, ++g) {
+                // a warp-wide look-up of the next 32 pages
+                const int k = (t - w.t0) & 31;
+                if (k == 0) {
+                    __syncwarp();
+                    const int i = t + lane;
+                    ids = i < w.t1 && i * kPage < w.len ? table[i] : 0;
+                    if (ids < 0 || ids >= p.num_pages) {
+                        record_error(&g_chunk_err, kErrPageOutOfRange, ids);
+                        ids = 0;
+                    }
+                }
+                const int page = __shfl_sync(0xffffffffu, ids, k);
+                if (lane == 0) {
+                    const int s = g % kStages, round = g / kStages;
+                    if (round > 0 && !mbar_wait_bounded(&empty[s], (round - 1) & 1)) {
+                        record_error(&g_chunk_err, kErrWaitTimeout, 22);
+                        ok = false;
+                    } else if (t * kPage < w.len) {
+                        uint8_t *stage = smem + SplitSmem::kRing + s * kStageBytes;
+                        mbar_arrive_expect_tx(&full[s], kStageBytes);
+                        const int row = (page * kNumKvHeads + w.kvh) * kPage;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) tma_load_2d(stage + c * 2048, &tmk, c * 64, row, &full[s], pol);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            tma_load_2d(stage + kTileBytes + c * 2048, &tmv, c * 64, row, &full[s], pol);
+                    } else {
+                        mbar_arrive(&full[s]);  // an empty cache: the tile is all masked
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0);
+            }
+            if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) || !walk_next<SplitTiling>(p.rag, w)) break;
+        }
+        return;
+    }
+
+    // ---------------------------------------------------------------- consumers
+    float *m_s = reinterpret_cast<float *>(smem + SplitSmem::kM);
+    float *l_s = reinterpret_cast<float *>(smem + SplitSmem::kL);
+    float *join = reinterpret_cast<float *>(smem + SplitSmem::kJoin);
+    const int r0 = lane >> 2;          // C-fragment rows r0 and r0 + 8
+    const int cpair = (lane & 3) * 2;  // C-fragment column pair
+    // ldmatrix lane roles: matrix mi = lane / 8, row-in-matrix = lane % 8
+    const int mi = lane >> 3;
+    const int k_tok = (mi >> 1) * 8 + (lane & 7);  // K: matrices (tok 0-7|8-15) x (k lo|hi)
+    const int k_dim_off = (mi & 1) * 8;
+    const int v_tok = (mi & 1) * 8 + (lane & 7);   // V: matrices (tok lo|hi) x (dim lo|hi)
+    const int v_dim_off = (mi >> 1) * 8;
+    auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(kConsumers * 32) : "memory"); };
+
+    int g0 = 0;  // the CTA's tiles before this unit
+    for (int unit = 0;; ++unit) {
+        const int n = w.n, L = w.len, nrows = n * kGroup, qb = unit & 1;
+        // visible token bound per C row: row j sees tokens < L - n + j + 1; rows of nobody see none
+        const int vis0 = r0 < nrows ? L - n + r0 / kGroup + 1 : 0;
+        const int vis1 = r0 + 8 < nrows ? L - n + (r0 + 8) / kGroup + 1 : 0;
+        const uint32_t q_base = smem_u32(smem + SplitSmem::kQ) + (qb * kRows + (lane & 15)) * kQRowBytes + (lane >> 4) * 16;
+        float o[32][4];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        // A wait that gives up is recorded and the warp runs on (every later wait is bounded too), so
+        // that the four warps stay in step at their barriers.
+        if (!mbar_wait_bounded(&q_full[qb], (unit >> 1) & 1)) record_error(&g_chunk_err, kErrWaitTimeout, 23);
+        int t = w.t0 + ((warp - g0) & (kConsumers - 1));  // this warp's first tile: (g0 + t - t0) % 4 == warp
+        for (; t < w.t1; t += kConsumers) {
+            const int g = g0 + t - w.t0;
+            const int s = g % kStages;
+            if (!mbar_wait_bounded(&full[s], (g / kStages) & 1)) {
+                record_error(&g_chunk_err, kErrWaitTimeout, 24);
+                break;
+            }
+            uint8_t *kt = smem + SplitSmem::kRing + s * kStageBytes;
+            uint8_t *vt = kt + kTileBytes;
+            const uint32_t k_base = smem_u32(kt);
+            const uint32_t v_base = smem_u32(vt);
+            const int tok0 = t * kPage;
+            const int nvalid = min(kPage, L - tok0);
+
+            // S[16 rows x 16 tokens] = Q K^T
+            float sacc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int kk = 0; kk < kHeadDim / 16; ++kk) {
+                uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
+                ldsm_x4(q_base + kk * 32, a0, a1, a2, a3);
+                ldsm_x4(k_base + swz_page_offset(k_tok, kk * 16 + k_dim_off), b0, b1, b2, b3);
+                mma_bf16_16816(sacc[0], a0, a1, a2, a3, b0, b1);
+                mma_bf16_16816(sacc[1], a0, a1, a2, a3, b2, b3);
+            }
+
+            // masked, log2-scaled scores; online softmax in registers
+            float sc[2][4];
+            float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int tk = tok0 + i * 8 + cpair + e;
+                    sc[i][e] = (tk < vis0) ? sacc[i][e] * p.scale_log2 : -INFINITY;
+                    sc[i][2 + e] = (tk < vis1) ? sacc[i][2 + e] * p.scale_log2 : -INFINITY;
+                    mx0 = fmaxf(mx0, sc[i][e]);
+                    mx1 = fmaxf(mx1, sc[i][2 + e]);
+                }
+            }
+            if (kScores) {
+                // the rows and lanes of a tile fill whole 32-byte sectors of [token][head]
+                float *s0 = p.scores + (((int64_t)(w.row0 + r0 / kGroup) * kNumKvHeads + w.kvh) * p.score_stride + tok0 + cpair) * kGroup + r0 % kGroup;
+                float *s1 = s0 + 2 * kNumKvHeads * p.score_stride * kGroup;  // row r0 + 8: two query tokens on
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int tk = tok0 + i * 8 + cpair + e;
+                        if (tk < vis0) s0[(i * 8 + e) * kGroup] = sc[i][e];
+                        if (tk < vis1) s1[(i * 8 + e) * kGroup] = sc[i][2 + e];
+                    }
+                }
+            }
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+            const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
+            const float mu0 = (mn0 == -INFINITY) ? 0.f : mn0;
+            const float mu1 = (mn1 == -INFINITY) ? 0.f : mn1;
+            const bool grow = mn0 != m0 || mn1 != m1;
+            const float corr0 = fast_exp2(m0 - mu0);  // m = -inf -> 0
+            const float corr1 = fast_exp2(m1 - mu1);
+            m0 = mn0;
+            m1 = mn1;
+            float ps0 = 0.f, ps1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    sc[i][e] = fast_exp2(sc[i][e] - mu0);
+                    sc[i][2 + e] = fast_exp2(sc[i][2 + e] - mu1);
+                    ps0 += sc[i][e];
+                    ps1 += sc[i][2 + e];
+                }
+            }
+            l0 = l0 * corr0 + ps0;
+            l1 = l1 * corr1 + ps1;
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    o[i][0] *= corr0;
+                    o[i][1] *= corr0;
+                    o[i][2] *= corr1;
+                    o[i][3] *= corr1;
+                }
+            }
+            const uint32_t pa0 = pack_bf16x2(sc[0][0], sc[0][1]);
+            const uint32_t pa1 = pack_bf16x2(sc[0][2], sc[0][3]);
+            const uint32_t pa2 = pack_bf16x2(sc[1][0], sc[1][1]);
+            const uint32_t pa3 = pack_bf16x2(sc[1][2], sc[1][3]);
+
+            if (nvalid < kPage) {
+                // Slots past the sequence end hold stale bytes; zero their V rows so that a NaN
+                // pattern cannot leak through a zero probability.
+                for (int idx = lane; idx < (kPage - nvalid) * 4 * 8; idx += 32) {
+                    const int row = nvalid + idx / 32;
+                    const int u = idx % 32;  // 4 boxes x 8 units of 16 B
+                    *reinterpret_cast<uint4 *>(vt + (u >> 3) * 2048 + row * 128 + (u & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();  // generic writes before any later async-proxy refill
+                __syncwarp();
+            }
+
+            // O[16 x 256] += P[16 x 16] V[16 x 256]
+#pragma unroll
+            for (int nd = 0; nd < 16; ++nd) {
+                uint32_t b0, b1, b2, b3;
+                ldsm_x4_trans(v_base + swz_page_offset(v_tok, nd * 16 + v_dim_off), b0, b1, b2, b3);
+                mma_bf16_16816(o[2 * nd], pa0, pa1, pa2, pa3, b0, b1);
+                mma_bf16_16816(o[2 * nd + 1], pa0, pa1, pa2, pa3, b2, b3);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
+        }
+
+        // ------------------------------------------------------------ join the 4 warp states
+        if (lane == 0) mbar_arrive(&q_empty[qb]);
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        if ((lane & 3) == 0) {
+            m_s[warp * kRows + r0] = m0;
+            l_s[warp * kRows + r0] = l0;
+            m_s[warp * kRows + r0 + 8] = m1;
+            l_s[warp * kRows + r0 + 8] = l1;
+        }
+        sync();
+        float ma0 = -INFINITY, ma1 = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < kConsumers; ++q) {
+            ma0 = fmaxf(ma0, m_s[q * kRows + r0]);
+            ma1 = fmaxf(ma1, m_s[q * kRows + r0 + 8]);
+        }
+        const float c0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - ma0);
+        const float c1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - ma1);
+        const bool whole = w.t0 == 0 && w.t1 == w.tiles;
+        const int slot = w.t0 > 0 ? 0 : 1;
+        if (!whole && threadIdx.x == 0) {
+            frag[slot].kvh = w.kvh;
+            frag[slot].qt = 0;
+            frag[slot].last = slot == 1 ? share_of_end(*line, index, w.tiles - w.t1) : 0;
+            frag[slot].seq = w.seq;
+        }
+        // rows of the join: 4, 8 or 16, so that its 16 KiB hold [4 warps][rows][cols]
+        const int jrows = nrows <= 4 ? 4 : nrows <= 8 ? 8 : 16;
+        const int cols = kJoinFloats / kConsumers / jrows;  // 256, 128 or 64
+        for (int d0 = 0; d0 < kHeadDim; d0 += cols) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const int d = i * 8 + cpair - d0;
+                if (i * 8 < d0 || i * 8 >= d0 + cols) continue;
+                if (r0 < jrows)
+                    *reinterpret_cast<float2 *>(&join[(warp * jrows + r0) * cols + d]) = make_float2(o[i][0] * c0, o[i][1] * c0);
+                if (r0 + 8 < jrows)
+                    *reinterpret_cast<float2 *>(&join[(warp * jrows + r0 + 8) * cols + d]) = make_float2(o[i][2] * c1, o[i][3] * c1);
+            }
+            sync();
+            for (int i = threadIdx.x; i < nrows * cols / 2; i += kConsumers * 32) {
+                const int r = i / (cols / 2), d = i % (cols / 2) * 2;
+                float2 acc = make_float2(0.f, 0.f);
+                float ma = -INFINITY, den = 0.f;
+#pragma unroll
+                for (int q = 0; q < kConsumers; ++q) {
+                    const float2 v = *reinterpret_cast<const float2 *>(&join[(q * jrows + r) * cols + d]);
+                    acc.x += v.x;
+                    acc.y += v.y;
+                    ma = fmaxf(ma, m_s[q * kRows + r]);
+                }
+#pragma unroll
+                for (int q = 0; q < kConsumers; ++q) {
+                    const float mq = m_s[q * kRows + r];
+                    if (mq != -INFINITY) den += l_s[q * kRows + r] * fast_exp2(mq - ma);
+                }
+                const int64_t row = (int64_t)(w.row0 + r / kGroup) * kNumQHeads + w.kvh * kGroup + r % kGroup;
+                if (!whole) {
+                    float *dst = p.parts + ((int64_t)(index * 2 + slot) * p.rag.max_q_len * kGroup + r) * kPartial;
+                    *reinterpret_cast<float2 *>(dst + 2 + d0 + d) = acc;
+                    if (d0 + d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(ma * kLn2, den);
+                    continue;
+                }
+                const float inv = den == 0.f ? 0.f : 1.f / den;
+                acc.x *= inv;
+                acc.y *= inv;
+                if (p.gate != nullptr) {
+                    const uint32_t gv = *reinterpret_cast<const uint32_t *>(p.gate + row * kHeadDim + d0 + d);
+                    acc.x = sigmoid_gate(acc.x, gv & 0xffffu);
+                    acc.y = sigmoid_gate(acc.y, gv >> 16);
+                }
+                *reinterpret_cast<uint32_t *>(p.out + row * kHeadDim + d0 + d) = pack_bf16x2(acc.x, acc.y);
+                if (d0 + d == 0 && p.lse != nullptr) p.lse[row] = den == 0.f ? -INFINITY : ma * kLn2 + logf(den);
+            }
+            sync();
+        }
+        g0 += w.t1 - w.t0;
+        if (!walk_next<SplitTiling>(p.rag, w)) break;
+    }
+}
+
+// The weights of 1024 tokens of one (sequence, kv head) from the scores that chunk_split_kernel left
+// and the rows' lse.
+struct AddParams {
+    RaggedBatch rag;
+    const float *lse;
+    const float *scores;
+    int64_t score_stride;
+    ChunkWeights w;
+};
+constexpr int kAddThreads = 256;
+constexpr int kAddTokens = 1024;
+
+__global__ void __launch_bounds__(kAddThreads) chunk_add_kernel(const AddParams p) {
+    pdl_trigger();
+    pdl_wait();
+    const int kvh = blockIdx.y, b = blockIdx.z;
+    const RaggedSeq sv = ragged_seq(p.rag, b, nullptr);
+    const int t0 = blockIdx.x * kAddTokens;
+    if (sv.n == 0 || t0 >= sv.len) return;
+    const int64_t slot = ragged_slot(p.w.slots, p.w.num_slots, b, blockIdx.x == 0 && kvh == 0 ? &g_chunk_err : nullptr);
+    if (slot < 0) return;
+    // log2 units; +inf for a row whose sum is 0, so that its -inf scores add nothing
+    float lse2[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        lse2[r] = INFINITY;
+        if (r < sv.n * kGroup) {
+            const float x = p.lse[(int64_t)(sv.row0 + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup];
+            if (x != -INFINITY) lse2[r] = x * kLog2e;
+        }
+    }
+    float *w = p.w.weights + (slot * kNumKvHeads + kvh) * p.w.stride;
+    const float4 *s = reinterpret_cast<const float4 *>(p.scores) + ((int64_t)sv.row0 * kNumKvHeads + kvh) * p.score_stride;
+#pragma unroll
+    for (int i = 0; i < kAddTokens / kAddThreads; ++i) {
+        const int t = t0 + i * kAddThreads + threadIdx.x;
+        if (t >= sv.len) break;
+        float add = 0.f;
+#pragma unroll
+        for (int j = 0; j < PGC_MAX_QUERIES; ++j) {
+            if (j >= sv.n || t > sv.len - sv.n + j) continue;  // not visible to row j
+            const float4 x = s[(int64_t)j * kNumKvHeads * p.score_stride + t];
+            add += fast_exp2(x.x - lse2[j * kGroup]);
+            add += fast_exp2(x.y - lse2[j * kGroup + 1]);
+            add += fast_exp2(x.z - lse2[j * kGroup + 2]);
+            add += fast_exp2(x.w - lse2[j * kGroup + 3]);
+        }
+        w[t] += add;
+    }
+}
+
+// =============================================================================================
+// More rows a sequence: two-SM tcgen05 kernel (cta_group::2). The tile of work and the roles are
+// those of the single-sequence prefill kernel: a cluster of two CTAs runs one kv head for 64 query
+// tokens (each CTA's 32 tokens x 4 GQA heads stacked into 128 rows, M = 256), each CTA stages its
+// own Q, 64 of a 128-key tile's keys and 128 of its value dims, S (two tiles) and O live in TMEM and
+// P is written over S. A share belongs to a pair, one pair per two SMs.
+// Loads, MMAs and softmax run on across units: the next unit's K, V and Q loads and its first S
+// products overlap this unit's last products and its epilogue.
+// =============================================================================================
+constexpr int kBM = 128;  // rows of a CTA: 32 tokens x 4 heads
+constexpr int kTokTile = 32;
+constexpr int kUnitTok = PairTiling::kTok;
+constexpr uint32_t kTmemCols = 512;
+constexpr float kLazyRescale = 8.0f;  // log2 units: rescale O only when the max grows by > 2^8
+constexpr int kSoftmaxWarps = 16;
+constexpr int kProducerWarps = 2;
+constexpr int kPairThreads = 32 * (kSoftmaxWarps + 1 + 2 * kProducerWarps);
+constexpr int kKeys = PairTiling::kKeys;      // keys per tile
+constexpr int kQBytes = kBM * kHeadDim * 2;   // [4 dim blocks][128 rows][128 B]
+constexpr int kKHalf = 64 * kHeadDim * 2;     // this CTA's 64 keys: [4][64][128 B]
+constexpr int kVHalf = kKeys * 128 * 2;       // this CTA's 128 dims: [2][128][128 B]
+constexpr int kKSlots = 3;
+constexpr int kVSlots = 2;
+constexpr uint32_t kTO = 0;    // O: 256 columns
+constexpr uint32_t kTS = 256;  // S tiles: 2 x 128 columns; P(j) over the first 64 of S(j)
+struct PairParams {
+    RaggedBatch rag;
+    const int32_t *block_tables;
+    int max_pages_per_seq;
+    int64_t num_pages;
+    const uint16_t *v_pages;
+    const uint16_t *gate;
+    uint16_t *out;
+    float *lse;
+    Fragment *frags;  // [pairs][2]
+    float *parts;     // [pairs][2][256][258]
+    float scale_log2;
+};
+
+struct PairSmem {
+    static constexpr int kQ = 0;
+    static constexpr int kK = kQ + kQBytes;
+    static constexpr int kV = kK + kKSlots * kKHalf;
+    static constexpr int kBar = kV + kVSlots * kVHalf;
+    // leader-side: q_full, k_full[3], v_full[2], p_full[2], o_free; both sides: q_empty, k_empty[3],
+    // v_empty[2], s_full[2], pv_done[2]
+    static constexpr int kNumBars = 2 + kKSlots + kVSlots + 2 + 1 + kKSlots + kVSlots + 2 + 2;
+    static constexpr int kRed = kBar + kNumBars * 8;
+    static constexpr int kWalk = kRed + 4 * kBM * 4;  // red: [4 key quarters][128 rows] fp32
+    static constexpr int kLine = kWalk + 48;
+    static constexpr int kTmemSlot = kLine + 16;
+    static constexpr int kAbort = kTmemSlot + 8;
+    static constexpr int kBytes = kAbort + 8;
+};
+static_assert(PairSmem::kWalk % 8 == 0, "walk slot");
+static_assert(PairSmem::kBytes <= 232448, "pair shared memory exceeds the sm_100 limit");
+static_assert(PGC_CHUNK_MAX_BATCH * 8 <= kKSlots * kKHalf, "the schedule's scratch is the K ring");
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     chunk_pair_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
@@ -388,8 +704,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const int lane = threadIdx.x & 31;
     const int pair = blockIdx.x >> 1;
 
-    const bool busy = find_share(p.rag, reinterpret_cast<int64_t *>(smem + PairSmem::kK), pair, gridDim.x >> 1, share,
-                                 blockIdx.x == 0 ? &g_chunk_err : nullptr);
+    Line *line = reinterpret_cast<Line *>(smem + PairSmem::kLine);
+    const bool busy = find_share<PairTiling>(p.rag, reinterpret_cast<int64_t *>(smem + PairSmem::kK), pair, gridDim.x >> 1,
+                                             share, line, blockIdx.x == 0 ? &g_chunk_err : nullptr);
     Fragment *frag = p.frags + pair * 2;
     if (leader && threadIdx.x < 2) frag[threadIdx.x].seq = -1;
     if (!busy) return;  // both CTAs of the pair
@@ -479,7 +796,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                             tma_load_2d_pair(dst + c * (64 * 128) + pp * 2048, &tmk, c * 64, row, kbar, pol);
                     }
                 }
-                if (!walk_next(p.rag, w)) break;
+                if (!walk_next<PairTiling>(p.rag, w)) break;
             }
         }
     } else if (warp >= kSoftmaxWarps + 1 + kProducerWarps) {
@@ -546,7 +863,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 }
                 __syncwarp();
             }
-            if (!walk_next(p.rag, w)) break;
+            if (!walk_next<PairTiling>(p.rag, w)) break;
         }
     } else if (warp == kSoftmaxWarps) {
         // ------------------------------------------------------------ pair MMA issuer (leader)
@@ -577,7 +894,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 ++ag;
                 if (++at == a.t1) {
                     umma2_commit_pair(q_empty);
-                    more = walk_next(p.rag, a);
+                    more = walk_next<PairTiling>(p.rag, a);
                     at = a.t0;
                     ++aunit;
                 }
@@ -607,7 +924,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     umma2_commit_pair(&v_empty[sl]);
                     umma2_commit_pair(&pv_done[b]);
                 }
-                if (!ok || !walk_next(p.rag, w)) break;
+                if (!ok || !walk_next<PairTiling>(p.rag, w)) break;
             }
         }
     } else {
@@ -710,7 +1027,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             if (!whole && leader && warp == 0 && lane == 0) {
                 frag[slot].kvh = w.kvh;
                 frag[slot].qt = w.qt;
-                frag[slot].last = w.t1 == w.tiles;
+                frag[slot].last = slot == 1 ? share_of_end(*line, pair, w.tiles - w.t1) : 0;
                 frag[slot].seq = w.seq;
             }
             if (live) {
@@ -771,7 +1088,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(obar);
-            if (!walk_next(p.rag, w)) break;
+            if (!walk_next<PairTiling>(p.rag, w)) break;
         }
     }
     // neither CTA may leave (or free TMEM) while the pair MMA or the peer can still touch it
@@ -783,154 +1100,186 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
 }
 
-// Joins the fragments of the units that were cut: block (p, y) takes the unit that pair p left
-// unfinished (its last fragment) and the first fragments of the pairs after it, up to the one that
-// holds the unit's last tile. A warp per row; lane l owns dims [8 l, 8 l + 8).
-constexpr int kMergeY = 16;
+// Joins the fragments of the units that were cut: blocks (p, *) take the unit that share p left
+// unfinished, its slot 1 there and slot 0 of the shares after it up to the one that ends it. A block
+// takes kRowsPerBlock rows, 8 / kRowsPerBlock warps a row (the fragments dealt to them in turn: a
+// single long sequence has 64 and more); lane l owns dims [8 l, 8 l + 8).
+struct MergeParams {
+    RaggedBatch rag;
+    const Fragment *frags;
+    const float *parts;  // [shares][2][rows][258]
+    int rows;            // of a fragment
+    int tok;             // query tokens of a unit
+    const uint16_t *gate;
+    uint16_t *out;
+    float *lse;
+};
 
-__global__ void __launch_bounds__(256) chunk_merge_kernel(const PairParams p) {
+template <int kRowsPerBlock>
+__global__ void __launch_bounds__(256) chunk_merge_kernel(const MergeParams p) {
+    constexpr int kSplit = 8 / kRowsPerBlock;  // warps a row
+    __shared__ float red[kRowsPerBlock][kSplit][kPartial];
     pdl_trigger();
     pdl_wait();
-    const int pair = blockIdx.x, pairs = gridDim.x;
-    const Fragment f = p.frags[pair * 2 + 1];
+    const int index = blockIdx.x;
+    const Fragment f = p.frags[index * 2 + 1];
     if (f.seq < 0) return;
-    int last = pair + 1;  // the pair whose first fragment ends the unit
-    while (last < pairs && p.frags[last * 2].seq == f.seq && !p.frags[last * 2].last) ++last;
-    if (last >= pairs) return;  // not reached: a cut unit is finished by a later pair
     const RaggedSeq sv = ragged_seq(p.rag, f.seq, nullptr);
-    const int lane = threadIdx.x & 31;
-    const int64_t slot_floats = (int64_t)2 * kBM * kPartial;
-    for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < 2 * kBM; r += kMergeY * 8) {
-        const int tok = f.qt * kUnitTok + r / kGroup;
-        if (tok >= sv.n) break;  // rows are in token order
-        const float *first = p.parts + (pair * 2 + 1) * slot_floats + (int64_t)r * kPartial;
-        const float *next = p.parts + (int64_t)(pair + 1) * 2 * slot_floats + (int64_t)r * kPartial;
-        const int np = last - pair;  // fragments behind the first, one every 2 slots
-        float ma = first[0];
-        for (int i = 0; i < np; ++i) ma = fmaxf(ma, next[i * 2 * slot_floats]);
-        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        float den = 0.f;
-        for (int i = -1; i < np; ++i) {
-            const float *pc = i < 0 ? first : next + i * 2 * slot_floats;
-            const float mc = pc[0];
-            if (mc == -INFINITY) continue;
-            const float w = exp2f((mc - ma) * kLog2e);
-            den += pc[1] * w;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int sub = warp % kSplit, rb = warp / kSplit;
+    const int r = blockIdx.y * kRowsPerBlock + rb;
+    const int tok = f.qt * p.tok + r / kGroup;
+    const bool live = r < p.rows && tok < sv.n;  // uniform in the warps of a row
+    const int64_t slot = (int64_t)p.rows * kPartial;
+    // fragment i: slot 1 of this share, then slot 0 of the next ones
+    const float *base = p.parts + index * 2 * slot + (int64_t)r * kPartial;
+    auto part = [&](int i) { return base + (i == 0 ? slot : i * 2 * slot); };
+    const int np = f.last - index + 1;
+    float ma = -INFINITY, den = 0.f;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (live) {
+        for (int i = lane; i < np; i += 32) ma = fmaxf(ma, part(i)[0]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, o));
+#pragma unroll 2
+        for (int i = sub; i < np; i += kSplit) {
+            const float *pc = part(i);
+            const float2 ml = *reinterpret_cast<const float2 *>(pc);
             const float2 *o = reinterpret_cast<const float2 *>(pc + 2 + 8 * lane);
+            const float2 v[4] = {o[0], o[1], o[2], o[3]};
+            const float w = ml.x == -INFINITY ? 0.f : exp2f((ml.x - ma) * kLog2e);
+            den += ml.y * w;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float2 v = o[k];
-                acc[2 * k] += v.x * w;
-                acc[2 * k + 1] += v.y * w;
+                acc[2 * k] += v[k].x * w;
+                acc[2 * k + 1] += v[k].y * w;
             }
         }
-        const int64_t orow = (int64_t)(sv.row0 + tok) * kNumQHeads + f.kvh * kGroup + r % kGroup;
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = (den == 0.f) ? 0.f : acc[k] / den;
-        if (p.gate != nullptr) {
-            const uint4 gq = *reinterpret_cast<const uint4 *>(p.gate + orow * kHeadDim + 8 * lane);
-            const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = sigmoid_gate(v[k], (gw[k >> 1] >> ((k & 1) * 16)) & 0xffffu);
-        }
-        uint4 q;
-        q.x = pack_bf16x2(v[0], v[1]);
-        q.y = pack_bf16x2(v[2], v[3]);
-        q.z = pack_bf16x2(v[4], v[5]);
-        q.w = pack_bf16x2(v[6], v[7]);
-        *reinterpret_cast<uint4 *>(p.out + orow * kHeadDim + 8 * lane) = q;
-        if (p.lse != nullptr && lane == 0) p.lse[orow] = (den == 0.f) ? -INFINITY : ma + logf(den);
     }
+    if (kSplit > 1) {
+        float *mine = red[rb][sub];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<float2 *>(mine + 2 + 8 * lane + 2 * k) = make_float2(acc[2 * k], acc[2 * k + 1]);
+        if (lane == 0) mine[0] = den;
+        __syncthreads();
+        if (sub != 0) return;
+#pragma unroll
+        for (int s = 1; s < kSplit; ++s) {
+            const float *other = red[rb][s];
+            den += other[0];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] += other[2 + 8 * lane + k];
+        }
+    }
+    if (!live) return;
+    const int64_t orow = (int64_t)(sv.row0 + tok) * kNumQHeads + f.kvh * kGroup + r % kGroup;
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = acc[k] * inv;
+    if (p.gate != nullptr) {
+        const uint4 gq = *reinterpret_cast<const uint4 *>(p.gate + orow * kHeadDim + 8 * lane);
+        const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = sigmoid_gate(v[k], (gw[k >> 1] >> ((k & 1) * 16)) & 0xffffu);
+    }
+    uint4 q;
+    q.x = pack_bf16x2(v[0], v[1]);
+    q.y = pack_bf16x2(v[2], v[3]);
+    q.z = pack_bf16x2(v[4], v[5]);
+    q.w = pack_bf16x2(v[6], v[7]);
+    *reinterpret_cast<uint4 *>(p.out + orow * kHeadDim + 8 * lane) = q;
+    if (p.lse != nullptr && lane == 0) p.lse[orow] = (den == 0.f) ? -INFINITY : ma + logf(den);
 }
 
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Workspace of a call, in order: partials; then, for the split form with weights, the scores; for
-// the pair form, the fragment records and, with weights and no caller's lse, the lse.
+// Workspace of a call: the shares' records and partials, with weights the rows' lse, and in the split
+// form the scores.
 struct Layout {
-    size_t parts = 0, scores = 0, frags = 0, lse = 0, total = 0;
+    bool split;
+    int shares, rows;  // rows of a partial
+    size_t frags = 0, parts = 0, lse = 0, scores = 0, total = 0;
     int64_t score_stride = 0;
 };
-Layout layout(int batch, int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count) {
+Layout layout(int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count) {
     Layout l;
-    size_t at = 0;
-    if (max_q_len <= PGC_MAX_QUERIES) {
-        const DecodePlan plan = decode_plan(batch, max_seq_len, sm_count);
-        l.parts = at;
-        at = align256(at + (size_t)total_q * kNumQHeads * plan.max_splits * kPartial * sizeof(float));
-        if (weights) {
-            l.score_stride = (max_seq_len + kPage - 1) / kPage * kPage;
-            l.scores = at;
-            at = align256(at + (size_t)total_q * kNumKvHeads * l.score_stride * kGroup * sizeof(float));
-        }
-    } else {
-        const size_t pairs = sm_count / 2;
-        l.parts = at;
-        at = align256(at + pairs * 2 * 2 * kBM * kPartial * sizeof(float));
-        l.frags = at;
-        at = align256(at + pairs * 2 * sizeof(Fragment));
-        if (weights) {
-            l.lse = at;
-            at = align256(at + (size_t)total_q * kNumQHeads * sizeof(float));
-        }
-    }
-    l.total = at;
+    l.split = max_q_len <= PGC_MAX_QUERIES;
+    l.shares = l.split ? 2 * sm_count : sm_count / 2;
+    l.rows = l.split ? max_q_len * kGroup : 2 * kBM;
+    l.parts = align256((size_t)l.shares * 2 * sizeof(Fragment));
+    l.lse = align256(l.parts + (size_t)l.shares * 2 * l.rows * kPartial * sizeof(float));
+    l.scores = align256(l.lse + (weights ? (size_t)total_q * kNumQHeads * sizeof(float) : 0));
+    l.score_stride = (max_seq_len + kPage - 1) / kPage * kPage;
+    l.total = l.scores;
+    if (weights && l.split) l.total += (size_t)total_q * kNumKvHeads * l.score_stride * kGroup * sizeof(float);
     return l;
 }
 
 }  // namespace
 
-size_t chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count) {
-    return layout(batch, total_q, max_q_len, max_seq_len, weights, sm_count).total;
+size_t chunk_workspace_bytes(int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count) {
+    return layout(total_q, max_q_len, max_seq_len, weights, sm_count).total;
 }
 
-cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtensorMap &tv, const uint16_t *k_pages,
-                         const uint16_t *v_pages, int64_t num_pages, const int32_t *block_tables,
-                         int max_pages_per_seq, const RaggedBatch &rag, float scale, const uint16_t *gate,
-                         uint16_t *out, float *lse, const ChunkWeights *weights, void *workspace, int sm_count,
-                         cudaStream_t stream) {
-    const Layout lay = layout(rag.batch, rag.total_q, rag.max_q_len, rag.max_seq_len, weights != nullptr, sm_count);
-    uint8_t *ws = static_cast<uint8_t *>(workspace);
-    float *parts = reinterpret_cast<float *>(ws + lay.parts);
-    if (rag.max_q_len <= PGC_MAX_QUERIES) {
-        float *scores = weights != nullptr ? reinterpret_cast<float *>(ws + lay.scores) : nullptr;
-        cudaError_t e = launch_ragged_split(q, tk, tv, num_pages, block_tables, max_pages_per_seq, rag, scale, parts,
-                                            scores, lay.score_stride, k_pages, v_pages, sm_count, stream);
-        if (e != cudaSuccess) return e;
-        FinishParams fp = {};
-        fp.rag = rag;
-        fp.parts = parts;
-        fp.max_splits = decode_plan(rag.batch, rag.max_seq_len, sm_count).max_splits;
-        fp.merge_blocks = rag.batch * rag.max_q_len * kNumQHeads * (kHeadDim / 32);
-        fp.gate = gate;
-        fp.out = out;
-        fp.lse = lse;
-        int blocks = fp.merge_blocks;
-        if (weights != nullptr) {
-            fp.scores = scores;
-            fp.score_stride = lay.score_stride;
-            fp.weights = weights->weights;
-            fp.weights_stride = weights->stride;
-            fp.num_slots = weights->num_slots;
-            fp.slots = weights->slots;
-            fp.add_chunks = (rag.max_seq_len + kAddTokens - 1) / kAddTokens;
-            blocks += rag.batch * kNumKvHeads * fp.add_chunks;
-        }
-        return launch_pdl(chunk_finish_kernel, dim3((unsigned)blocks), dim3(kFinishThreads), 0, stream, fp);
-    }
+cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtensorMap &tv, const uint16_t *v_pages,
+                         int64_t num_pages, const int32_t *block_tables, int max_pages_per_seq,
+                         const RaggedBatch &rag, float scale, const uint16_t *gate, uint16_t *out, float *lse,
+                         const ChunkWeights *weights, void *workspace, int sm_count, cudaStream_t stream) {
     static std::atomic<bool> attr_set[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(chunk_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             PairSmem::kBytes);
+        const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+        cudaError_t e = cudaFuncSetAttribute(chunk_pair_kernel, attr, PairSmem::kBytes);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_split_kernel<false>, attr, kSplitSmem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_split_kernel<true>, attr, kSplitSmem);
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) attr_set[dev] = true;
     }
+    const Layout lay = layout(rag.total_q, rag.max_q_len, rag.max_seq_len, weights != nullptr, sm_count);
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    if (lse == nullptr && weights != nullptr) lse = reinterpret_cast<float *>(ws + lay.lse);
+    MergeParams mp = {};
+    mp.rag = rag;
+    mp.frags = reinterpret_cast<const Fragment *>(ws + lay.frags);
+    mp.parts = reinterpret_cast<const float *>(ws + lay.parts);
+    mp.rows = lay.rows;
+    mp.gate = gate;
+    mp.out = out;
+    mp.lse = lse;
+    if (lay.split) {
+        SplitParams sp = {};
+        sp.rag = rag;
+        sp.q = q;
+        sp.block_tables = block_tables;
+        sp.max_pages_per_seq = max_pages_per_seq;
+        sp.num_pages = num_pages;
+        sp.gate = gate;
+        sp.out = out;
+        sp.lse = lse;
+        sp.frags = reinterpret_cast<Fragment *>(ws + lay.frags);
+        sp.parts = reinterpret_cast<float *>(ws + lay.parts);
+        sp.scores = weights != nullptr ? reinterpret_cast<float *>(ws + lay.scores) : nullptr;
+        sp.score_stride = lay.score_stride;
+        sp.scale_log2 = scale * kLog2e;
+        const dim3 grid(lay.shares), block(kSplitThreads);
+        cudaError_t e = weights != nullptr ? launch_pdl(chunk_split_kernel<true>, grid, block, kSplitSmem, stream, tk, tv, sp)
+                                           : launch_pdl(chunk_split_kernel<false>, grid, block, kSplitSmem, stream, tk, tv, sp);
+        mp.tok = SplitTiling::kTok;
+        if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel<1>, dim3(lay.shares, lay.rows), dim3(256), 0, stream, mp);
+        if (e != cudaSuccess || weights == nullptr) return e;
+        AddParams ap = {};
+        ap.rag = rag;
+        ap.lse = lse;
+        ap.scores = sp.scores;
+        ap.score_stride = lay.score_stride;
+        ap.w = *weights;
+        return launch_pdl(chunk_add_kernel, dim3((rag.max_seq_len + kAddTokens - 1) / kAddTokens, kNumKvHeads, rag.batch),
+                          dim3(kAddThreads), 0, stream, ap);
+    }
     CUtensorMap tq;
     if (q_tensor_map(q, rag.total_q, &tq) != PGC_OK) return cudaErrorInvalidValue;
-    const int pairs = sm_count / 2;
     PairParams pp = {};
     pp.rag = rag;
     pp.block_tables = block_tables;
@@ -939,15 +1288,15 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
     pp.v_pages = v_pages;
     pp.gate = gate;
     pp.out = out;
-    pp.lse = lse != nullptr || weights == nullptr ? lse : reinterpret_cast<float *>(ws + lay.lse);
+    pp.lse = lse;
     pp.frags = reinterpret_cast<Fragment *>(ws + lay.frags);
-    pp.parts = parts;
+    pp.parts = reinterpret_cast<float *>(ws + lay.parts);
     pp.scale_log2 = scale * kLog2e;
-    cudaError_t e = launch_pdl(chunk_pair_kernel, dim3(2 * pairs), dim3(kPairThreads), PairSmem::kBytes, stream, tq, tk, tv, pp);
-    if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel, dim3(pairs, kMergeY), dim3(256), 0, stream, pp);
+    cudaError_t e = launch_pdl(chunk_pair_kernel, dim3(2 * lay.shares), dim3(kPairThreads), PairSmem::kBytes, stream, tq, tk, tv, pp);
+    mp.tok = PairTiling::kTok;
+    if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel<8>, dim3(lay.shares, lay.rows / 8), dim3(256), 0, stream, mp);
     if (e != cudaSuccess || weights == nullptr) return e;
-    return launch_chunk_weights(tq, tk, num_pages, block_tables, max_pages_per_seq, rag, scale, pp.lse, *weights,
-                                sm_count, stream);
+    return launch_chunk_weights(tq, tk, num_pages, block_tables, max_pages_per_seq, rag, scale, lse, *weights, sm_count, stream);
 }
 
 cudaError_t chunk_read_error(DevErrorHost *e, bool clear) {

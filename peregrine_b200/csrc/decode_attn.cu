@@ -22,7 +22,6 @@
 
 #include "pgc_common.cuh"
 #include "pgc_internal.h"
-#include "pgc_ragged.cuh"
 
 namespace pgc {
 
@@ -64,11 +63,6 @@ struct SplitParams {
     // coherently through L2); `prefetch_ahead` pages past the ring while streaming.
     int prefetch_pre, prefetch_ahead;
     const uint8_t *k_base, *v_base;
-    // ragged batch (pgc_chunk_attn at up to 4 queries a sequence): the sequences' query rows and
-    // lengths come from `rag`; row = query row * 16 + head
-    RaggedBatch rag;
-    float *scores;         // nullable: [total_q][4 kv heads][score_stride][4 heads] log2-scaled scores
-    int64_t score_stride;  // tokens
 };
 
 struct SmemLayout {
@@ -86,10 +80,7 @@ __device__ __forceinline__ void prefetch_l2(const void *ptr, uint32_t bytes) {
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ptr), "r"(bytes) : "memory");
 }
 
-// kRagged: every sequence has its own number of query rows (SplitParams::rag); kScores: the scaled
-// scores of the visible tokens are stored too, 16 B per query row, kv head and token against the
-// 1 KiB of K and V read for it, so that the received-attention weights need no second pass over K.
-template <bool kFused, bool kRagged = false, bool kScores = false>
+template <bool kFused>
 __global__ void __launch_bounds__(kThreads, 2)
     decode_split_kernel(const __grid_constant__ CUtensorMap tmk,
                         const __grid_constant__ CUtensorMap tmv, const SplitParams p) {
@@ -101,6 +92,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int split = blockIdx.x;
     const int kvh = blockIdx.y;
     const int seq = blockIdx.z;
+    const int nq = p.num_queries;
+    const int nrows = nq * kGroup;
 
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + SmemLayout::kBarOff);
     uint64_t *empty = full + kStages;
@@ -119,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        if (kFused) mbar_init(kv_ready, p.num_queries);
+        if (kFused) mbar_init(kv_ready, nq);
         fence_mbar_init();
     }
     if (threadIdx.x == kConsumers * 32) {
@@ -129,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         // stream drains (its tail and the merge before this launch): page ids outside the pool
         // are skipped, so a stale table costs bandwidth, never correctness.
         if (p.prefetch_pre > 0) {
-            const int Lg = kRagged ? min(p.seq_lens[seq], p.rag.max_seq_len) : p.seq_lens[seq];
+            const int Lg = p.seq_lens[seq];
             const int tb = split * p.pages_per_split * kPage;
             if (tb < Lg) {
                 const int np = min(p.prefetch_pre, (min(Lg, tb + p.pages_per_split * kPage) - tb + kPage - 1) / kPage);
@@ -146,23 +139,14 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
     }
     pdl_wait();
-    RaggedSeq sv = {};
-    if (kRagged) {
-        sv = ragged_seq(p.rag, seq, threadIdx.x == 0 && kvh == 0 && split == 0 ? &g_decode_err : nullptr);
-        if (sv.n == 0) return;  // no query rows (uniform across the CTA)
-    }
-    const int L = kRagged ? sv.len : p.seq_lens[seq];
-    const int nq = kRagged ? sv.n : p.num_queries;
-    const int nrows = nq * kGroup;
-    // query row of token j
-    auto row_of = [&](int j) -> int64_t { return kRagged ? sv.row0 + j : seq * nq + j; };
+    const int L = p.seq_lens[seq];
     const int tok_begin = split * p.pages_per_split * kPage;
     if (tok_begin >= L) {
         // A split past the sequence end leaves an empty partial (m = -inf, l = 0; its o is never
         // summed), so the merges take every planned split without reading the lengths again.
         if (threadIdx.x < nrows) {
             const int j = threadIdx.x / kGroup, g = threadIdx.x % kGroup;
-            const int64_t row = row_of(j) * kNumQHeads + kvh * kGroup + g;
+            const int64_t row = (int64_t)(seq * nq + j) * kNumQHeads + kvh * kGroup + g;
             float *dst = p.ws + (row * p.max_splits + split) * kPartial;
             dst[0] = -INFINITY;
             dst[1] = 0.f;
@@ -246,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (r < nrows) {
                 const int j = r / kGroup, g = r % kGroup;
                 const uint16_t *src =
-                    p.q + (row_of(j) * kNumQHeads + kvh * kGroup + g) * kHeadDim;
+                    p.q + ((int64_t)(seq * nq + j) * kNumQHeads + kvh * kGroup + g) * kHeadDim;
                 v = reinterpret_cast<const uint4 *>(src)[c];
             }
             *reinterpret_cast<uint4 *>(q_s + r * kQRowBytes + c * 16) = v;
@@ -414,21 +398,6 @@ __global__ void __launch_bounds__(kThreads, 2)
                 mx1 = fmaxf(mx1, sc[n][2 + e]);
             }
         }
-        if (kScores) {
-            // the four lanes of a row and its neighbours' rows fill whole 32-byte sectors of
-            // [token][head]
-            float *s0 = p.scores + ((row_of(r0 / kGroup) * kNumKvHeads + kvh) * p.score_stride + tok0 + cpair) * kGroup + r0 % kGroup;
-            float *s1 = s0 + 2 * kNumKvHeads * p.score_stride * kGroup;  // row r0 + 8: two query tokens on
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int t = tok0 + n * 8 + cpair + e;
-                    if (r0 < nrows && t < vis0) s0[(n * 8 + e) * kGroup] = sc[n][e];
-                    if (r0 + 8 < nrows && t < vis1) s1[(n * 8 + e) * kGroup] = sc[n][2 + e];
-                }
-            }
-        }
         mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
         mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
         mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
@@ -535,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             den += l_s[w * 16 + r] * wt[w];
         }
         const int j = r / kGroup, g = r % kGroup;
-        const int64_t row = row_of(j) * kNumQHeads + kvh * kGroup + g;
+        const int64_t row = (int64_t)(seq * nq + j) * kNumQHeads + kvh * kGroup + g;
         float *dst = p.ws + (row * p.max_splits + split) * kPartial;
         for (int d = tid; d < kHeadDim; d += kConsumers * 32) {
             float acc = 0.f;
@@ -806,44 +775,6 @@ cudaError_t launch_decode(const uint16_t *q, const CUtensorMap &tk, const CUtens
     const int64_t rows = (int64_t)batch * num_queries * kNumQHeads;
     return launch_pdl(merge_kernel, dim3((unsigned)rows, kHeadDim / 32), dim3(kMergeWarps * 32), 0,
                       stream, mp);
-}
-
-cudaError_t launch_ragged_split(const uint16_t *q, const CUtensorMap &tk, const CUtensorMap &tv,
-                                int64_t num_pages, const int32_t *block_tables, int max_pages_per_seq,
-                                const RaggedBatch &rag, float scale, float *parts, float *scores,
-                                int64_t score_stride, const void *k_pages, const void *v_pages,
-                                int sm_count, cudaStream_t stream) {
-    auto plain = decode_split_kernel<false, true, false>;
-    auto scored = decode_split_kernel<false, true, true>;
-    static std::atomic<bool> attr_set[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(plain, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(scored, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-        if (e != cudaSuccess) return e;
-        if (dev >= 0 && dev < 64) attr_set[dev] = true;
-    }
-    const DecodePlan plan = decode_plan(rag.batch, rag.max_seq_len, sm_count);
-    SplitParams sp = {};
-    sp.q = q;
-    sp.block_tables = block_tables;
-    sp.seq_lens = rag.seq_lens;
-    sp.ws = parts;
-    sp.num_pages = num_pages;
-    sp.max_pages_per_seq = max_pages_per_seq;
-    sp.pages_per_split = plan.pages_per_split;
-    sp.max_splits = plan.max_splits;
-    sp.scale_log2 = scale * kLog2e;
-    sp.prefetch_pre = plan.prefetch_pre;
-    sp.prefetch_ahead = plan.prefetch_ahead;
-    sp.k_base = static_cast<const uint8_t *>(k_pages);
-    sp.v_base = static_cast<const uint8_t *>(v_pages);
-    sp.rag = rag;
-    sp.scores = scores;
-    sp.score_stride = score_stride;
-    const dim3 grid(plan.max_splits, kNumKvHeads, rag.batch);
-    return launch_pdl(scores != nullptr ? scored : plain, grid, dim3(kThreads), kSmemBytes, stream, tk, tv, sp);
 }
 
 cudaError_t launch_merge_partials(const float *partials, int64_t rows, int num_parts,

@@ -78,13 +78,6 @@ cudaError_t launch_merge_partials(const float *partials, int64_t rows, int num_p
                                   int64_t part_stride, const uint16_t *gate, uint16_t *out,
                                   cudaStream_t stream);
 cudaError_t decode_read_error(DevErrorHost *e, bool clear);
-// the split kernel over a ragged batch of at most PGC_MAX_QUERIES rows a sequence: partials
-// [total_q * 16][decode_plan().max_splits][258]; scores nullable
-cudaError_t launch_ragged_split(const uint16_t *q, const CUtensorMap &tk, const CUtensorMap &tv,
-                                int64_t num_pages, const int32_t *block_tables, int max_pages_per_seq,
-                                const RaggedBatch &rag, float scale, float *parts, float *scores,
-                                int64_t score_stride, const void *k_pages, const void *v_pages,
-                                int sm_count, cudaStream_t stream);
 // context-parallel exchange buffer: [2][world][16][8][34] u64 epoch-tagged words
 size_t cp_buffer_bytes(int world);
 cudaError_t launch_cp_decode(const uint16_t *q, const CUtensorMap &tk, const CUtensorMap &tv,
@@ -139,12 +132,11 @@ struct ChunkWeights {
     int64_t stride, num_slots;
     const int32_t *slots;  // [batch], nullable
 };
-size_t chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count);
-cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtensorMap &tv, const uint16_t *k_pages,
-                         const uint16_t *v_pages, int64_t num_pages, const int32_t *block_tables,
-                         int max_pages_per_seq, const RaggedBatch &rag, float scale, const uint16_t *gate,
-                         uint16_t *out, float *lse, const ChunkWeights *weights, void *workspace, int sm_count,
-                         cudaStream_t stream);
+size_t chunk_workspace_bytes(int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count);
+cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtensorMap &tv, const uint16_t *v_pages,
+                         int64_t num_pages, const int32_t *block_tables, int max_pages_per_seq,
+                         const RaggedBatch &rag, float scale, const uint16_t *gate, uint16_t *out, float *lse,
+                         const ChunkWeights *weights, void *workspace, int sm_count, cudaStream_t stream);
 cudaError_t chunk_read_error(DevErrorHost *e, bool clear);
 
 // chunk_weights.cu: weights += column sums of exp(scale q.k - lse) over the batch's rows

@@ -35,7 +35,7 @@ def chunk(lib, with_weights, **change):
     (dict(pages=0), INVALID), (dict(batch=-1), INVALID), (dict(rows=-1), INVALID), (dict(qmax=-1), INVALID),
     (dict(lmax=-1), INVALID), (dict(lmax=0), INVALID), (dict(width=-1), INVALID), (dict(width=0), INVALID),
     (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID), (dict(batch=4097, num_slots=5000), BOUNDS),
-    (dict(width=9), BOUNDS), (dict(pages=1 << 25), BOUNDS), (dict(rows=(1 << 24) + 1), BOUNDS),
+    (dict(width=9), BOUNDS), (dict(pages=1 << 25), BOUNDS), (dict(rows=(1 << 22) + 1), BOUNDS),
     (dict(lmax=(1 << 24) + 1, width=1 << 21, stride=1 << 25), BOUNDS), (dict(ws_bytes=0), WORKSPACE),
     (dict(q=A + 8), ALIGN), (dict(k=A + 2), ALIGN), (dict(v=A + 4), ALIGN), (dict(gate=A + 8), ALIGN),
     (dict(out=A + 2), ALIGN), (dict(ws=A + 4), ALIGN), (dict(lse=A + 2), ALIGN),
@@ -57,7 +57,7 @@ def test_workspace_is_required_in_full(lib, qmax, weights):
     need = lib.pgc_chunk_workspace_bytes(2, 8, qmax, 160, weights)
     assert need > 0
     assert chunk(lib, bool(weights), qmax=qmax, ws_bytes=need - 1) == WORKSPACE
-    for bad in ((0, 8, 4, 160), (4097, 8, 4, 160), (2, 0, 4, 160), (2, (1 << 24) + 1, 4, 160), (2, 8, 0, 160),
+    for bad in ((0, 8, 4, 160), (4097, 8, 4, 160), (2, 0, 4, 160), (2, (1 << 22) + 1, 4, 160), (2, 8, 0, 160),
                 (2, 8, 4, 0), (2, 8, 4, (1 << 24) + 1)):
         assert lib.pgc_chunk_workspace_bytes(*bad, weights) == 0
 
@@ -65,7 +65,9 @@ def test_workspace_is_required_in_full(lib, qmax, weights):
 def test_workspace_grows_with_the_shape(lib):
     f = lib.pgc_chunk_workspace_bytes
     assert f(2, 8, 4, 160, 1) > f(2, 8, 4, 160, 0)
-    assert f(2, 8, 4, 1 << 15, 1) - f(2, 8, 4, 1 << 15, 0) == 8 * 4 * (1 << 15) * 4 * 4
+    scores, lse = 8 * 4 * (1 << 15) * 4 * 4, 8 * 16 * 4
+    assert f(2, 8, 4, 1 << 15, 1) - f(2, 8, 4, 1 << 15, 0) == scores + lse
+    assert f(2, 8, 4, 1 << 20, 0) == f(4096, 1 << 12, 4, 100, 0) <= 10 << 20
     assert f(4096, 1 << 20, 512, 1 << 20, 0) == f(1, 5, 5, 100, 0) <= 38 << 20
 
 
