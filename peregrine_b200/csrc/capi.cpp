@@ -461,7 +461,7 @@ static bool chunk_shape_ok(int batch, int total_q, int max_q_len, int max_seq_le
 
 size_t pgc_chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_seq_len, int with_weights) {
     if (!chunk_shape_ok(batch, total_q, max_q_len, max_seq_len)) return 0;
-    return chunk_workspace_bytes(total_q, max_q_len, max_seq_len, with_weights != 0, current_sm_count());
+    return chunk_workspace_bytes(batch, total_q, max_q_len, max_seq_len, with_weights != 0, current_sm_count());
 }
 
 static int chunk_call(const uint16_t *q, const uint16_t *k_pages, const uint16_t *v_pages, int64_t num_pages,
@@ -488,7 +488,7 @@ static int chunk_call(const uint16_t *q, const uint16_t *k_pages, const uint16_t
         ((uintptr_t)lse & 3u) != 0 || (weights && ((uintptr_t)weights->weights & 3u) != 0))
         return PGC_ERR_ALIGN;
     const int sms = current_sm_count();
-    if (!workspace || workspace_bytes < chunk_workspace_bytes(total_q, max_q_len, max_seq_len,
+    if (!workspace || workspace_bytes < chunk_workspace_bytes(batch, total_q, max_q_len, max_seq_len,
                                                               weights != nullptr, sms))
         return PGC_ERR_WORKSPACE;
     int st = check_device(nullptr);

@@ -39,11 +39,13 @@ __device__ __forceinline__ float sigmoid_gate(float v, uint32_t gate_bits) {
 // =============================================================================================
 struct PairTiling {
     static constexpr int kTok = 64, kKeys = 128;
+    static constexpr bool kWarpScan = false;
     // A share below this many tiles costs more in its Q load, pipeline fill and partials than it saves.
     static constexpr int kMinShare = 4;
 };
 struct SplitTiling {
     static constexpr int kTok = PGC_MAX_QUERIES, kKeys = kPage;
+    static constexpr bool kWarpScan = true;
     static constexpr int kMinShare = 4;
 };
 
@@ -95,37 +97,120 @@ __device__ __forceinline__ bool walk_next(const RaggedBatch &rag, Walk &w) {
     return true;
 }
 
-// The line's length and the shares it is cut into: share p is tiles [total * p / shares, total *
-// (p + 1) / shares).
+// The line's length and the shares it is cut into: the first `longer` ones take base + 1 tiles, the
+// others base.
 struct Line {
-    int64_t total;
-    int shares;
+    int64_t total, base;
+    int shares, longer;
 };
 
-// Share `index` of a grid of `grid`, which uses min(grid, total / kMinShare) of them. Run by the whole
-// CTA; `cost` is scratch (one int64 per sequence). Returns false when the share is empty.
+// 64-bit quotients of non-negative numbers, in 32 bits where they fit (the 64-bit division is a few
+// hundred cycles on the way to the first load).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+    return a / b;
+}
+template <class T>
+__device__ __forceinline__ Line make_line(int64_t total, int grid) {
+    Line l;
+    const int64_t w = quotient(total, T::kMinShare);
+    l.total = total;
+    l.shares = w < 1 ? 1 : w > grid ? grid : (int)w;
+    l.base = quotient(total, l.shares);
+    l.longer = (int)(total - l.base * l.shares);
+    return l;
+}
+__device__ __forceinline__ int64_t share_begin(const Line &l, int index) { return l.base * index + min(index, l.longer); }
+__device__ __forceinline__ int share_of(const Line &l, int64_t tile) {
+    const int64_t cut = (l.base + 1) * l.longer;
+    return tile < cut ? (int)quotient(tile, l.base + 1) : l.longer + (int)quotient(tile - cut, l.base);
+}
+
+// Start of the walk: `off` tiles into sequence wk.seq, whose kv heads have `per` tiles each.
+template <class T>
+__device__ __forceinline__ void walk_start(Walk &wk, int64_t off, int64_t per, int64_t left) {
+    wk.kvh = (int)quotient(off, per);
+    off -= wk.kvh * per;
+    for (wk.qt = 0;; ++wk.qt) {
+        const int t = unit_tiles<T>(wk.n, wk.len, wk.qt);
+        if (off < t) break;
+        off -= t;
+    }
+    wk.left = (int)left;  // a grid of shares keeps it within int (PGC_CHUNK_MAX_ROWS)
+    walk_unit<T>(wk, (int)off);
+}
+template <class T>
+__device__ __forceinline__ int64_t seq_cost(const RaggedSeq &s) {  // of one kv head
+    if (s.n <= T::kTok) return s.n == 0 ? 0 : unit_tiles<T>(s.n, s.len, 0);
+    int64_t c = 0;
+    for (int qt = 0; qt * T::kTok < s.n; ++qt) c += unit_tiles<T>(s.n, s.len, qt);
+    return c;
+}
+
+// Share `index` of a grid of `grid`. Run by the whole CTA; `line` (shared memory) is written by thread
+// 0, `out` is shared memory that the larger batches go through, `cost` their scratch (one int64 per
+// sequence). Returns false when the share is empty. With kWarpScan batches of up to 128 sequences are scanned by every warp for itself,
+// which needs no barrier: 1.5 us off a single sequence's decode (in the pair kernel the registers that it
+// takes cost 2 % of the main loop).
 template <class T>
 __device__ __forceinline__ bool find_share(const RaggedBatch &rag, int64_t *cost, int index, int grid, Walk *out,
-                                           Line *line, DevError *err) {
-    for (int b = threadIdx.x; b < rag.batch; b += blockDim.x) {
-        const RaggedSeq s = ragged_seq(rag, b, err);
-        int64_t c = 0;
-        for (int qt = 0; qt * T::kTok < s.n; ++qt) c += unit_tiles<T>(s.n, s.len, qt);
-        cost[b] = c * kNumKvHeads;
+                                           Line *line, DevError *err, Walk &wk) {
+    constexpr int kChunks = 4;
+    const int lane = threadIdx.x & 31;
+    wk.seq = -1;
+    if (T::kWarpScan && rag.batch <= 32 * kChunks) {
+        // a sequence has at most 2^22 tiles (PGC_CHUNK_MAX_TOKENS), so 32 bits hold the line
+        RaggedSeq s[kChunks];
+        int c[kChunks], incl[kChunks], total = 0;
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+            s[k] = RaggedSeq{0, 0, 0};
+            if (k * 32 + lane < rag.batch) s[k] = ragged_seq(rag, k * 32 + lane, threadIdx.x < 32 ? err : nullptr);
+            c[k] = incl[k] = 0;
+        }
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+            if (k * 32 >= rag.batch) break;
+            c[k] = (int)seq_cost<T>(s[k]) * kNumKvHeads;
+            incl[k] = c[k];
+#pragma unroll 1
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl[k], o);
+                if (lane >= o) incl[k] += v;
+            }
+            incl[k] += total;
+            total = __shfl_sync(0xffffffffu, incl[k], 31);
+        }
+        const Line ln = make_line<T>(total, grid);
+        if (threadIdx.x == 0) *line = ln;
+        const int begin = (int)share_begin(ln, index), end = (int)share_begin(ln, index + 1);
+        if (index >= ln.shares || end <= begin) return false;
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+            const uint32_t hit = __ballot_sync(0xffffffffu, incl[k] > begin);
+            if (hit == 0) continue;
+            const int src = __ffs(hit) - 1;
+            wk.seq = k * 32 + src;
+            wk.row0 = __shfl_sync(0xffffffffu, s[k].row0, src);
+            wk.n = __shfl_sync(0xffffffffu, s[k].n, src);
+            wk.len = __shfl_sync(0xffffffffu, s[k].len, src);
+            const int all = __shfl_sync(0xffffffffu, c[k], src);
+            const int before = __shfl_sync(0xffffffffu, incl[k], src) - all;
+            walk_start<T>(wk, begin - before, all / kNumKvHeads, end - begin);
+            break;
+        }
+        return true;
     }
+    for (int b = threadIdx.x; b < rag.batch; b += blockDim.x) cost[b] = seq_cost<T>(ragged_seq(rag, b, err)) * kNumKvHeads;
     __syncthreads();
     if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
         int64_t total = 0;
         for (int b = lane; b < rag.batch; b += 32) total += cost[b];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        int64_t w = total / T::kMinShare;
-        w = w < 1 ? 1 : w > grid ? grid : w;
-        const int64_t begin = total * index / w, end = total * (index + 1) / w;
-        Walk wk = {};
-        wk.seq = -1;
-        if (index < w && end > begin) {
+        const Line ln = make_line<T>(total, grid);
+        const int64_t begin = share_begin(ln, index), end = share_begin(ln, index + 1);
+        if (index < ln.shares && end > begin) {
             int64_t before = 0;
             for (int b0 = 0; b0 < rag.batch; b0 += 32) {
                 const int64_t c = b0 + lane < rag.batch ? cost[b0 + lane] : 0;
@@ -145,39 +230,31 @@ __device__ __forceinline__ bool find_share(const RaggedBatch &rag, int64_t *cost
                 before += __shfl_sync(0xffffffffu, incl, 31);
             }
             walk_seq(rag, wk);
-            const int64_t per = cost[wk.seq] / kNumKvHeads;
-            int64_t off = begin - before;
-            wk.kvh = (int)(off / per);
-            off -= wk.kvh * per;
-            for (wk.qt = 0;; ++wk.qt) {
-                const int t = unit_tiles<T>(wk.n, wk.len, wk.qt);
-                if (off < t) break;
-                off -= t;
-            }
-            wk.left = (int)(end - begin);  // a grid of shares keeps it within int (PGC_CHUNK_MAX_ROWS)
-            walk_unit<T>(wk, (int)off);
+            walk_start<T>(wk, begin - before, cost[wk.seq] / kNumKvHeads, end - begin);
         }
         if (lane == 0) {
             *out = wk;
-            line->total = total;
-            line->shares = (int)w;
+            *line = ln;
         }
     }
     __syncthreads();
-    return out->seq >= 0;
+    wk = *out;
+    return wk.seq >= 0;
 }
 
-// A cut unit's record: slot 0 of a share is the unit that its start cuts, slot 1 the one that its end
-// cuts. Slot 1 names the share that ends the unit; the shares between hold its middle in their slot 0.
+// Where a unit is cut: a share leaves the unit that its start cuts in its slot 0 of the partials and
+// the unit that only its end cuts in its slot 1. The unit goes on in slot 0 of the shares behind. The
+// share with its first tile writes the unit's record.
 struct Fragment {
-    int seq;  // -1: none
-    int kvh, qt;
-    int last;  // slot 1: the share with the unit's last tile
+    int first, last;  // the shares with the unit's first and last tile; equal: not cut
+    int row;          // the unit's first query row
+    int rows_kvh;     // its query rows * 4 + kv head
 };
-// `at`: the unit's tiles behind the share, which ends at total * (index + 1) / shares.
-__device__ __forceinline__ int share_of_end(const Line &line, int index, int64_t behind) {
-    const int64_t x = line.total * (index + 1) / line.shares + behind - 1;  // the unit's last tile
-    return (int)(((x + 1) * line.shares - 1) / line.total);
+template <class T>
+__device__ __forceinline__ void write_record(Fragment *f, const Walk &w, const Line &l, int index) {
+    const int last = w.t1 < w.tiles ? share_of(l, share_begin(l, index + 1) + (w.tiles - w.t1) - 1) : index;
+    *reinterpret_cast<int4 *>(f) = make_int4(index, last, w.row0 + w.qt * T::kTok,
+                                             min(T::kTok, w.n - w.qt * T::kTok) * kNumKvHeads + w.kvh);
 }
 
 // =============================================================================================
@@ -196,7 +273,7 @@ constexpr int kTileBytes = kPage * kHeadDim * 2;  // one (page, kv head) of K or
 constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kRows = PGC_MAX_QUERIES * kGroup;
 constexpr int kQRowBytes = kHeadDim * 2 + 16;  // padded row: conflict-free ldmatrix
-constexpr int kJoinFloats = 4096;              // the warps' states are joined 16 KiB at a time
+constexpr int kJoinPitch = kHeadDim + 8;       // floats of a joined row, padded: conflict-free float2 stores
 
 struct SplitParams {
     RaggedBatch rag;
@@ -207,7 +284,7 @@ struct SplitParams {
     const uint16_t *gate;
     uint16_t *out;
     float *lse;        // nullable
-    Fragment *frags;   // [shares][2]
+    Fragment *frags;   // [batch][4]
     float *parts;      // [shares][2][4 * max_q_len][258]
     float *scores;     // nullable: [total_q][4][score_stride][4], scaled by log2(e)
     int64_t score_stride;
@@ -218,16 +295,17 @@ struct SplitSmem {
     static constexpr int kRing = 0;  // 1024-aligned
     static constexpr int kQ = kRing + kStages * kStageBytes;
     static constexpr int kJoin = kQ + 2 * kRows * kQRowBytes;
-    static constexpr int kM = kJoin + kJoinFloats * 4;  // [4 warps][16 rows]
+    static constexpr int kM = kJoin + kConsumers * 4 * kJoinPitch * 4;  // [4 warps][16 rows]
     static constexpr int kL = kM + kConsumers * kRows * 4;
     static constexpr int kBar = kL + kConsumers * kRows * 4;  // full[4], empty[4], q_full[2], q_empty[2]
     static constexpr int kWalk = kBar + (2 * kStages + 4) * 8;
     static constexpr int kLine = kWalk + 48;
-    static constexpr int kBytes = kLine + 16;
+    static constexpr int kBytes = kLine + 24;
 };
 constexpr int kSplitSmem = SplitSmem::kBytes + 1024;  // + alignment slack
-static_assert(sizeof(Walk) <= 48 && sizeof(Line) <= 16, "schedule slots");
+static_assert(sizeof(Walk) <= 48 && sizeof(Line) <= 24 && SplitSmem::kWalk % 8 == 0, "schedule slots");
 static_assert(PGC_CHUNK_MAX_BATCH * 8 <= kStages * kStageBytes, "the schedule's scratch is the ring");
+static_assert(kConsumers * kRows * kJoinPitch * 4 <= SplitSmem::kJoin, "the last join's scratch is the ring and Q");
 
 // Untiled bulk copy global -> shared, completion bytes on `bar`; 16-byte aligned, a multiple of 16.
 __device__ __forceinline__ void bulk_load(void *smem_dst, const void *src, uint32_t bytes, uint64_t *bar) {
@@ -246,11 +324,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     uint64_t *empty = full + kStages;
     uint64_t *q_full = empty + kStages;
     uint64_t *q_empty = q_full + 2;
-    Walk *share = reinterpret_cast<Walk *>(smem + SplitSmem::kWalk);
-    Line *line = reinterpret_cast<Line *>(smem + SplitSmem::kLine);
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const int index = blockIdx.x;
+    Line *line = reinterpret_cast<Line *>(smem + SplitSmem::kLine);
 
     pdl_trigger();
     if (threadIdx.x == 0) {
@@ -267,14 +344,14 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         tma_prefetch_desc(&tmv);
     }
     pdl_wait();
-    Fragment *frag = p.frags + index * 2;
-    if (threadIdx.x < 2) frag[threadIdx.x].seq = -1;
+    Walk w;
     const bool busy = find_share<SplitTiling>(p.rag, reinterpret_cast<int64_t *>(smem + SplitSmem::kRing), index,
-                                              gridDim.x, share, line, index == 0 ? &g_chunk_err : nullptr);
+                                              gridDim.x, reinterpret_cast<Walk *>(smem + SplitSmem::kWalk),
+                                              line,
+                                              index == 0 ? &g_chunk_err : nullptr, w);
     if (!busy) return;
     fence_proxy_async_smem();  // the schedule's scratch becomes the ring
     __syncthreads();
-    Walk w = *share;
 
     if (warp == kConsumers) {
         // ------------------------------------------------------------ producer
@@ -488,9 +565,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
         if ((lane & 3) == 0) {
             m_s[warp * kRows + r0] = m0;
-            l_s[warp * kRows + r0] = l0;
             m_s[warp * kRows + r0 + 8] = m1;
-            l_s[warp * kRows + r0 + 8] = l1;
         }
         sync();
         float ma0 = -INFINITY, ma1 = -INFINITY;
@@ -501,117 +576,90 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         }
         const float c0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - ma0);
         const float c1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - ma1);
+        // the sums on the common maximum, read behind the next barrier
+        if ((lane & 3) == 0) {
+            l_s[warp * kRows + r0] = l0 * c0;
+            l_s[warp * kRows + r0 + 8] = l1 * c1;
+        }
         const bool whole = w.t0 == 0 && w.t1 == w.tiles;
-        const int slot = w.t0 > 0 ? 0 : 1;
-        if (!whole && threadIdx.x == 0) {
-            frag[slot].kvh = w.kvh;
-            frag[slot].qt = 0;
-            frag[slot].last = slot == 1 ? share_of_end(*line, index, w.tiles - w.t1) : 0;
-            frag[slot].seq = w.seq;
-        }
-        // rows of the join: 4, 8 or 16, so that its 16 KiB hold [4 warps][rows][cols]
-        const int jrows = nrows <= 4 ? 4 : nrows <= 8 ? 8 : 16;
-        const int cols = kJoinFloats / kConsumers / jrows;  // 256, 128 or 64
-        for (int d0 = 0; d0 < kHeadDim; d0 += cols) {
+        float *part = p.parts + (int64_t)(index * 2 + (w.t0 > 0 ? 0 : 1)) * p.rag.max_q_len * kGroup * kPartial;
+        // dims d, d + 1 of row r
+        auto emit = [&](int r, int d, float2 acc) {
+            const float den = (l_s[r] + l_s[kRows + r]) + (l_s[2 * kRows + r] + l_s[3 * kRows + r]);
+            const float ma = fmaxf(fmaxf(m_s[r], m_s[kRows + r]), fmaxf(m_s[2 * kRows + r], m_s[3 * kRows + r]));
+            if (!whole) {
+                float *dst = part + r * kPartial;
+                *reinterpret_cast<float2 *>(dst + 2 + d) = acc;
+                if (d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(ma * kLn2, den);
+                return;
+            }
+            const int64_t row = (int64_t)(w.row0 + r / kGroup) * kNumQHeads + w.kvh * kGroup + r % kGroup;
+            const float inv = den == 0.f ? 0.f : 1.f / den;
+            acc.x *= inv;
+            acc.y *= inv;
+            if (p.gate != nullptr) {
+                const uint32_t gv = *reinterpret_cast<const uint32_t *>(p.gate + row * kHeadDim + d);
+                acc.x = sigmoid_gate(acc.x, gv & 0xffffu);
+                acc.y = sigmoid_gate(acc.y, gv >> 16);
+            }
+            *reinterpret_cast<uint32_t *>(p.out + row * kHeadDim + d) = pack_bf16x2(acc.x, acc.y);
+            if (d == 0 && p.lse != nullptr) p.lse[row] = den == 0.f ? -INFINITY : ma * kLn2 + logf(den);
+        };
+        // the share's last unit: the ring and Q are free, and hold all rows at once
+        const bool last = w.left == w.t1 - w.t0;
+        if (nrows <= 4 || last) {
+            // one round: [4 warps][4, 8 or 16 rows][256 dims]
+            float *buf = nrows <= 4 ? join : reinterpret_cast<float *>(smem);
+            const int jrows = nrows <= 4 ? 4 : nrows <= 8 ? 8 : 16;
+            float *to = buf + (warp * jrows + r0) * kJoinPitch + cpair;
+            if (r0 < nrows) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const int d = i * 8 + cpair - d0;
-                if (i * 8 < d0 || i * 8 >= d0 + cols) continue;
-                if (r0 < jrows)
-                    *reinterpret_cast<float2 *>(&join[(warp * jrows + r0) * cols + d]) = make_float2(o[i][0] * c0, o[i][1] * c0);
-                if (r0 + 8 < jrows)
-                    *reinterpret_cast<float2 *>(&join[(warp * jrows + r0 + 8) * cols + d]) = make_float2(o[i][2] * c1, o[i][3] * c1);
+                for (int i = 0; i < 32; ++i) *reinterpret_cast<float2 *>(to + i * 8) = make_float2(o[i][0] * c0, o[i][1] * c0);
+            }
+            if (r0 + 8 < nrows) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    *reinterpret_cast<float2 *>(to + 8 * kJoinPitch + i * 8) = make_float2(o[i][2] * c1, o[i][3] * c1);
             }
             sync();
-            for (int i = threadIdx.x; i < nrows * cols / 2; i += kConsumers * 32) {
-                const int r = i / (cols / 2), d = i % (cols / 2) * 2;
+#pragma unroll 4
+            for (int r = 0; r < nrows; ++r) {
                 float2 acc = make_float2(0.f, 0.f);
-                float ma = -INFINITY, den = 0.f;
 #pragma unroll
-                for (int q = 0; q < kConsumers; ++q) {
-                    const float2 v = *reinterpret_cast<const float2 *>(&join[(q * jrows + r) * cols + d]);
-                    acc.x += v.x;
-                    acc.y += v.y;
-                    ma = fmaxf(ma, m_s[q * kRows + r]);
-                }
-#pragma unroll
-                for (int q = 0; q < kConsumers; ++q) {
-                    const float mq = m_s[q * kRows + r];
-                    if (mq != -INFINITY) den += l_s[q * kRows + r] * fast_exp2(mq - ma);
-                }
-                const int64_t row = (int64_t)(w.row0 + r / kGroup) * kNumQHeads + w.kvh * kGroup + r % kGroup;
-                if (!whole) {
-                    float *dst = p.parts + ((int64_t)(index * 2 + slot) * p.rag.max_q_len * kGroup + r) * kPartial;
-                    *reinterpret_cast<float2 *>(dst + 2 + d0 + d) = acc;
-                    if (d0 + d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(ma * kLn2, den);
-                    continue;
-                }
-                const float inv = den == 0.f ? 0.f : 1.f / den;
-                acc.x *= inv;
-                acc.y *= inv;
-                if (p.gate != nullptr) {
-                    const uint32_t gv = *reinterpret_cast<const uint32_t *>(p.gate + row * kHeadDim + d0 + d);
-                    acc.x = sigmoid_gate(acc.x, gv & 0xffffu);
-                    acc.y = sigmoid_gate(acc.y, gv >> 16);
-                }
-                *reinterpret_cast<uint32_t *>(p.out + row * kHeadDim + d0 + d) = pack_bf16x2(acc.x, acc.y);
-                if (d0 + d == 0 && p.lse != nullptr) p.lse[row] = den == 0.f ? -INFINITY : ma * kLn2 + logf(den);
+                for (int q = 0; q < kConsumers; ++q)
+                    acc = __fadd2_rn(acc, *reinterpret_cast<const float2 *>(&buf[(q * jrows + r) * kJoinPitch + 2 * threadIdx.x]));
+                emit(r, 2 * threadIdx.x, acc);
+            }
+            if (last) {
+                if (threadIdx.x == 0 && w.t0 == 0) write_record<SplitTiling>(&p.frags[w.seq * kNumKvHeads + w.kvh], w, *line, index);
+                return;
             }
             sync();
+        } else {
+            // four rounds of 64 dims: [4 warps][16 rows][64 dims]
+#pragma unroll
+            for (int round = 0; round < 4; ++round) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float *to = &join[(warp * 16 + r0) * (kJoinPitch / 4) + i * 8 + cpair];
+                    *reinterpret_cast<float2 *>(to) = make_float2(o[round * 8 + i][0] * c0, o[round * 8 + i][1] * c0);
+                    *reinterpret_cast<float2 *>(to + 8 * (kJoinPitch / 4)) = make_float2(o[round * 8 + i][2] * c1, o[round * 8 + i][3] * c1);
+                }
+                sync();
+                for (int i = threadIdx.x; i < nrows * 32; i += kConsumers * 32) {
+                    const int r = i >> 5, d = (i & 31) * 2;
+                    float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int q = 0; q < kConsumers; ++q)
+                        acc = __fadd2_rn(acc, *reinterpret_cast<const float2 *>(&join[(q * 16 + r) * (kJoinPitch / 4) + d]));
+                    emit(r, round * 64 + d, acc);
+                }
+                sync();
+            }
         }
+        if (threadIdx.x == 0 && w.t0 == 0) write_record<SplitTiling>(&p.frags[w.seq * kNumKvHeads + w.kvh], w, *line, index);
         g0 += w.t1 - w.t0;
-        if (!walk_next<SplitTiling>(p.rag, w)) break;
-    }
-}
-
-// The weights of 1024 tokens of one (sequence, kv head) from the scores that chunk_split_kernel left
-// and the rows' lse.
-struct AddParams {
-    RaggedBatch rag;
-    const float *lse;
-    const float *scores;
-    int64_t score_stride;
-    ChunkWeights w;
-};
-constexpr int kAddThreads = 256;
-constexpr int kAddTokens = 1024;
-
-__global__ void __launch_bounds__(kAddThreads) chunk_add_kernel(const AddParams p) {
-    pdl_trigger();
-    pdl_wait();
-    const int kvh = blockIdx.y, b = blockIdx.z;
-    const RaggedSeq sv = ragged_seq(p.rag, b, nullptr);
-    const int t0 = blockIdx.x * kAddTokens;
-    if (sv.n == 0 || t0 >= sv.len) return;
-    const int64_t slot = ragged_slot(p.w.slots, p.w.num_slots, b, blockIdx.x == 0 && kvh == 0 ? &g_chunk_err : nullptr);
-    if (slot < 0) return;
-    // log2 units; +inf for a row whose sum is 0, so that its -inf scores add nothing
-    float lse2[kRows];
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-        lse2[r] = INFINITY;
-        if (r < sv.n * kGroup) {
-            const float x = p.lse[(int64_t)(sv.row0 + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup];
-            if (x != -INFINITY) lse2[r] = x * kLog2e;
-        }
-    }
-    float *w = p.w.weights + (slot * kNumKvHeads + kvh) * p.w.stride;
-    const float4 *s = reinterpret_cast<const float4 *>(p.scores) + ((int64_t)sv.row0 * kNumKvHeads + kvh) * p.score_stride;
-#pragma unroll
-    for (int i = 0; i < kAddTokens / kAddThreads; ++i) {
-        const int t = t0 + i * kAddThreads + threadIdx.x;
-        if (t >= sv.len) break;
-        float add = 0.f;
-#pragma unroll
-        for (int j = 0; j < PGC_MAX_QUERIES; ++j) {
-            if (j >= sv.n || t > sv.len - sv.n + j) continue;  // not visible to row j
-            const float4 x = s[(int64_t)j * kNumKvHeads * p.score_stride + t];
-            add += fast_exp2(x.x - lse2[j * kGroup]);
-            add += fast_exp2(x.y - lse2[j * kGroup + 1]);
-            add += fast_exp2(x.z - lse2[j * kGroup + 2]);
-            add += fast_exp2(x.w - lse2[j * kGroup + 3]);
-        }
-        w[t] += add;
+        walk_next<SplitTiling>(p.rag, w);  // there is one: the last unit returned above
     }
 }
 
@@ -649,7 +697,7 @@ struct PairParams {
     const uint16_t *gate;
     uint16_t *out;
     float *lse;
-    Fragment *frags;  // [pairs][2]
+    Fragment *frags;  // [pairs]
     float *parts;     // [pairs][2][256][258]
     float scale_log2;
 };
@@ -665,7 +713,7 @@ struct PairSmem {
     static constexpr int kRed = kBar + kNumBars * 8;
     static constexpr int kWalk = kRed + 4 * kBM * 4;  // red: [4 key quarters][128 rows] fp32
     static constexpr int kLine = kWalk + 48;
-    static constexpr int kTmemSlot = kLine + 16;
+    static constexpr int kTmemSlot = kLine + 24;
     static constexpr int kAbort = kTmemSlot + 8;
     static constexpr int kBytes = kAbort + 8;
 };
@@ -698,17 +746,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     uint64_t *s_full = v_empty + kVSlots;   // each [2]
     uint64_t *pv_done = s_full + 2;         // each [2]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + PairSmem::kTmemSlot);
-    Walk *share = reinterpret_cast<Walk *>(smem + PairSmem::kWalk);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + PairSmem::kAbort);
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const int pair = blockIdx.x >> 1;
-
     Line *line = reinterpret_cast<Line *>(smem + PairSmem::kLine);
+
+    Walk w;
     const bool busy = find_share<PairTiling>(p.rag, reinterpret_cast<int64_t *>(smem + PairSmem::kK), pair, gridDim.x >> 1,
-                                             share, line, blockIdx.x == 0 ? &g_chunk_err : nullptr);
-    Fragment *frag = p.frags + pair * 2;
-    if (leader && threadIdx.x < 2) frag[threadIdx.x].seq = -1;
+                                             reinterpret_cast<Walk *>(smem + PairSmem::kWalk),
+                                             line,
+                                             blockIdx.x == 0 ? &g_chunk_err : nullptr, w);
+    // the record of the share, that no unit is cut by its end until its walk has ended
+    if (leader && threadIdx.x == 0) p.frags[pair].last = p.frags[pair].first = 0;
     if (!busy) return;  // both CTAs of the pair
     if (threadIdx.x == 0) {
         *abort_flag = 0;
@@ -751,7 +801,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         record_error(&g_chunk_err, kErrPageOutOfRange, page);
         return 0;
     };
-    Walk w = *share;
 
     if (warp >= kSoftmaxWarps + 1 && warp < kSoftmaxWarps + 1 + kProducerWarps) {
         // ------------------------------------------------------------ TMA: Q and this CTA's K half
@@ -1024,12 +1073,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             tc_fence_after();
             const bool whole = w.t0 == 0 && w.t1 == w.tiles;
             const int slot = w.t0 > 0 ? 0 : 1;
-            if (!whole && leader && warp == 0 && lane == 0) {
-                frag[slot].kvh = w.kvh;
-                frag[slot].qt = w.qt;
-                frag[slot].last = slot == 1 ? share_of_end(*line, pair, w.tiles - w.t1) : 0;
-                frag[slot].seq = w.seq;
-            }
             if (live) {
                 red[cg * kBM + r] = l;
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + qd) : "memory");
@@ -1090,6 +1133,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             if (lane == 0) mbar_arrive_cluster(obar);
             if (!walk_next<PairTiling>(p.rag, w)) break;
         }
+        if (leader && threadIdx.x == 0 && w.t0 == 0) write_record<PairTiling>(&p.frags[pair], w, *line, pair);
     }
     // neither CTA may leave (or free TMEM) while the pair MMA or the peer can still touch it
     tc_fence_before();
@@ -1100,79 +1144,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
 }
 
-// Joins the fragments of the units that were cut: blocks (p, *) take the unit that share p left
-// unfinished, its slot 1 there and slot 0 of the shares after it up to the one that ends it. A block
-// takes kRowsPerBlock rows, 8 / kRowsPerBlock warps a row (the fragments dealt to them in turn: a
-// single long sequence has 64 and more); lane l owns dims [8 l, 8 l + 8).
-struct MergeParams {
-    RaggedBatch rag;
+// =============================================================================================
+// The end of a call: joins the fragments of the units that were cut and, behind the split kernel, adds
+// the weights.
+// =============================================================================================
+constexpr int kFinishThreads = 512;
+constexpr int kFinishWarps = kFinishThreads / 32;
+constexpr int kAddTokens = 2048;
+
+struct FinishParams {
     const Fragment *frags;
     const float *parts;  // [shares][2][rows][258]
-    int rows;            // of a fragment
-    int tok;             // query tokens of a unit
+    int records;
+    int rows;          // of a fragment
+    int merge_blocks;  // the blocks behind them add weights
     const uint16_t *gate;
     uint16_t *out;
     float *lse;
+    RaggedBatch rag;  // the split form's: its records are by (sequence, kv head)
+    const float *scores;
+    int64_t score_stride;
+    ChunkWeights w;
+    int add_chunks;  // blocks per (sequence, kv head)
 };
 
-template <int kRowsPerBlock>
-__global__ void __launch_bounds__(256) chunk_merge_kernel(const MergeParams p) {
-    constexpr int kSplit = 8 / kRowsPerBlock;  // warps a row
-    __shared__ float red[kRowsPerBlock][kSplit][kPartial];
+__device__ __forceinline__ Fragment read_record(const FinishParams &p, int i) {
+    const int4 f = *reinterpret_cast<const int4 *>(&p.frags[i]);
+    return Fragment{f.x, f.y, f.z, f.w};
+}
+// Floats from a row's first fragment (slot 1 of the first share) to its fragment i (slot 0 of share
+// first + i), over a base at slot 0 of the first share.
+__device__ __forceinline__ int64_t fragment_at(const FinishParams &p, int i) {
+    return (int64_t)(i == 0 ? 1 : 2 * i) * p.rows * kPartial;
+}
+
+// Behind the pair kernel: blocks (share, rows / 16), a warp per row; lane l owns dims [8 l, 8 l + 8).
+__global__ void __launch_bounds__(kFinishThreads) chunk_merge_kernel(const FinishParams p) {
     pdl_trigger();
     pdl_wait();
-    const int index = blockIdx.x;
-    const Fragment f = p.frags[index * 2 + 1];
-    if (f.seq < 0) return;
-    const RaggedSeq sv = ragged_seq(p.rag, f.seq, nullptr);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int sub = warp % kSplit, rb = warp / kSplit;
-    const int r = blockIdx.y * kRowsPerBlock + rb;
-    const int tok = f.qt * p.tok + r / kGroup;
-    const bool live = r < p.rows && tok < sv.n;  // uniform in the warps of a row
-    const int64_t slot = (int64_t)p.rows * kPartial;
-    // fragment i: slot 1 of this share, then slot 0 of the next ones
-    const float *base = p.parts + index * 2 * slot + (int64_t)r * kPartial;
-    auto part = [&](int i) { return base + (i == 0 ? slot : i * 2 * slot); };
-    const int np = f.last - index + 1;
+    const Fragment f = read_record(p, blockIdx.x);
+    const int lane = threadIdx.x & 31;
+    const int r = blockIdx.y * kFinishWarps + (threadIdx.x >> 5);
+    const int kvh = f.rows_kvh % kNumKvHeads;
+    if (f.first >= f.last || r >= f.rows_kvh / kNumKvHeads * kGroup) return;
+    const float *base = p.parts + (int64_t)f.first * 2 * p.rows * kPartial + (int64_t)r * kPartial;
+    const int np = f.last - f.first + 1;
     float ma = -INFINITY, den = 0.f;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live) {
-        for (int i = lane; i < np; i += 32) ma = fmaxf(ma, part(i)[0]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, o));
 #pragma unroll 2
-        for (int i = sub; i < np; i += kSplit) {
-            const float *pc = part(i);
-            const float2 ml = *reinterpret_cast<const float2 *>(pc);
-            const float2 *o = reinterpret_cast<const float2 *>(pc + 2 + 8 * lane);
-            const float2 v[4] = {o[0], o[1], o[2], o[3]};
-            const float w = ml.x == -INFINITY ? 0.f : exp2f((ml.x - ma) * kLog2e);
-            den += ml.y * w;
+    for (int i = 0; i < np; ++i) {
+        const float *pc = base + fragment_at(p, i);
+        const float2 ml = *reinterpret_cast<const float2 *>(pc);
+        const float2 *o = reinterpret_cast<const float2 *>(pc + 2 + 8 * lane);
+        const float2 v[4] = {o[0], o[1], o[2], o[3]};
+        const float mx = fmaxf(ma, ml.x);
+        if (ml.x == -INFINITY) continue;  // the fragment saw nothing
+        const float corr = exp2f((ma - mx) * kLog2e), w = exp2f((ml.x - mx) * kLog2e);
+        ma = mx;
+        den = den * corr + ml.y * w;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                acc[2 * k] += v[k].x * w;
-                acc[2 * k + 1] += v[k].y * w;
-            }
+        for (int k = 0; k < 4; ++k) {
+            acc[2 * k] = acc[2 * k] * corr + v[k].x * w;
+            acc[2 * k + 1] = acc[2 * k + 1] * corr + v[k].y * w;
         }
     }
-    if (kSplit > 1) {
-        float *mine = red[rb][sub];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) *reinterpret_cast<float2 *>(mine + 2 + 8 * lane + 2 * k) = make_float2(acc[2 * k], acc[2 * k + 1]);
-        if (lane == 0) mine[0] = den;
-        __syncthreads();
-        if (sub != 0) return;
-#pragma unroll
-        for (int s = 1; s < kSplit; ++s) {
-            const float *other = red[rb][s];
-            den += other[0];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) acc[k] += other[2 + 8 * lane + k];
-        }
-    }
-    if (!live) return;
-    const int64_t orow = (int64_t)(sv.row0 + tok) * kNumQHeads + f.kvh * kGroup + r % kGroup;
+    const int64_t orow = (int64_t)(f.row + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup;
     const float inv = den == 0.f ? 0.f : 1.f / den;
     float v[8];
 #pragma unroll
@@ -1192,22 +1228,189 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const MergeParams p) {
     if (p.lse != nullptr && lane == 0) p.lse[orow] = (den == 0.f) ? -INFINITY : ma + logf(den);
 }
 
+// One row of a cut unit behind the split kernel, by a block: the fragments (64 and more of a single long
+// sequence) are dealt to the warps, four loads of a warp in flight, and the warps' sums joined in
+// shared memory. Short straight code: these few blocks run once, so they wait for instructions and
+// loads, not for arithmetic.
+__device__ __forceinline__ void merge_row(const FinishParams &p, const Fragment &f, int r) {
+    __shared__ float2 red_ml[kFinishWarps];
+    __shared__ float red[kFinishWarps][kHeadDim + 8];
+    constexpr int kBatch = 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int kvh = f.rows_kvh % kNumKvHeads;
+    if (r >= f.rows_kvh / kNumKvHeads * kGroup) return;  // uniform
+    const float *base = p.parts + (int64_t)f.first * 2 * p.rows * kPartial + (int64_t)r * kPartial;
+    const int np = f.last - f.first + 1;
+    float ma = -INFINITY, den = 0.f;
+    float2 acc[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = make_float2(0.f, 0.f);
+    for (int i0 = warp; i0 < np; i0 += kFinishWarps * kBatch) {
+        float2 ml[kBatch], v[kBatch][4];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            // past the last fragment: the first of this warp again, with weight 0
+            const int i = i0 + j * kFinishWarps;
+            const float *pc = base + fragment_at(p, i < np ? i : i0);
+            ml[j] = *reinterpret_cast<const float2 *>(pc);
+            if (i >= np) ml[j].x = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[j][k] = *reinterpret_cast<const float2 *>(pc + 2 + 2 * lane + 64 * k);
+        }
+        float mx = ma;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) mx = fmaxf(mx, ml[j].x);
+        const float base_m = mx == -INFINITY ? 0.f : mx;
+        const float corr = fast_exp2((ma - base_m) * kLog2e);
+        ma = mx;
+        den *= corr;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] = __fmul2_rn(acc[k], make_float2(corr, corr));
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const float w = fast_exp2((ml[j].x - base_m) * kLog2e);
+            den += ml[j].x == -INFINITY ? 0.f : ml[j].y * w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[k] = __ffma2_rn(v[j][k], make_float2(w, w), acc[k]);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) *reinterpret_cast<float2 *>(&red[warp][2 * lane + 64 * k]) = acc[k];
+    if (lane == 0) red_ml[warp] = make_float2(ma, den);
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= kHeadDim) return;
+    const int64_t orow = (int64_t)(f.row + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup;
+    const float gate = p.gate != nullptr ? sigmoid_gate(1.f, p.gate[orow * kHeadDim + d]) : 1.f;
+    // lane w: warp w's statistics
+    const float2 mine = lane < kFinishWarps ? red_ml[lane] : make_float2(-INFINITY, 0.f);
+    float mx = mine.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float scale = mine.x == -INFINITY ? 0.f : fast_exp2((mine.x - mx) * kLog2e);
+    den = mine.y * scale;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFinishWarps; ++w) sum += red[w][d] * __shfl_sync(0xffffffffu, scale, w);
+    const float o = den == 0.f ? 0.f : sum / den * gate;
+    p.out[orow * kHeadDim + d] = f32_to_bf16_bits(o);
+    if (p.lse != nullptr && d == 0) p.lse[orow] = (den == 0.f) ? -INFINITY : mx + logf(den);
+}
+
+// The weights of 2048 tokens of one (sequence, kv head) from the scores that the split kernel left and
+// the rows' lse: the split kernel's, or for a cut unit formed from the fragments' (m, l) here, so that
+// these blocks need not wait for the merging ones.
+__device__ __forceinline__ void add_weights(const FinishParams &p, int blk) {
+    __shared__ float lse2[kRows];  // log2 units
+    const int chunk = blk % p.add_chunks, unit = blk / p.add_chunks;
+    const int kvh = unit % kNumKvHeads, b = unit / kNumKvHeads;
+    const Fragment f = read_record(p, unit);  // of a sequence with rows only
+    const RaggedSeq sv = ragged_seq(p.rag, b, nullptr);
+    const int t0 = chunk * kAddTokens;
+    if (sv.n == 0 || t0 >= sv.len) return;
+    const int64_t slot = ragged_slot(p.w.slots, p.w.num_slots, b, chunk == 0 && kvh == 0 ? &g_chunk_err : nullptr);
+    if (slot < 0) return;
+    float *w = p.w.weights + (slot * kNumKvHeads + kvh) * p.w.stride;
+    const float4 *s = reinterpret_cast<const float4 *>(p.scores) + ((int64_t)sv.row0 * kNumKvHeads + kvh) * p.score_stride;
+    constexpr int kEach = kAddTokens / kFinishThreads;
+    float sum[kEach];
+    float4 x[kEach];
+    auto load_scores = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int t = t0 + i * kFinishThreads + threadIdx.x;
+            x[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (t <= sv.len - sv.n + j) x[i] = s[(int64_t)j * kNumKvHeads * p.score_stride + t];  // visible to row j
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int t = t0 + i * kFinishThreads + threadIdx.x;
+        sum[i] = t < sv.len ? w[t] : 0.f;
+    }
+    load_scores(0);
+    {
+        // 16 threads a row (the first half of the block); +inf for a row whose sum is 0, so that its -inf scores add nothing
+        const int r = threadIdx.x >> 4, lane16 = threadIdx.x & 15;
+        const bool mine = r < sv.n * kGroup;  // sv.n <= 4
+        float m = -INFINITY, l = 0.f;
+        if (f.first < f.last) {
+            const float *base = p.parts + (int64_t)f.first * 2 * p.rows * kPartial + (int64_t)r * kPartial;
+            const int np = mine ? f.last - f.first + 1 : 0;
+            for (int i = lane16; i < np; i += 16) {
+                const float2 ml = *reinterpret_cast<const float2 *>(base + fragment_at(p, i));
+                const float mx = fmaxf(m, ml.x);
+                if (mx == -INFINITY) continue;
+                l = l * exp2f((m - mx) * kLog2e) + ml.y * exp2f((ml.x - mx) * kLog2e);
+                m = mx;
+            }
+            float mx = m;
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            l = m == -INFINITY ? 0.f : l * exp2f((m - mx) * kLog2e);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            if (lane16 == 0 && r < kRows) lse2[r] = l == 0.f ? INFINITY : mx * kLog2e + log2f(l);
+        } else if (lane16 == 0 && r < kRows) {
+            lse2[r] = INFINITY;
+            if (mine) {
+                const float v = p.lse[(int64_t)(sv.row0 + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup];
+                if (v != -INFINITY) lse2[r] = v * kLog2e;
+            }
+        }
+    }
+    __syncthreads();
+    for (int j = 0;;) {
+        const float4 l = *reinterpret_cast<const float4 *>(&lse2[j * kGroup]);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            sum[i] += (fast_exp2(x[i].x - l.x) + fast_exp2(x[i].y - l.y)) + (fast_exp2(x[i].z - l.z) + fast_exp2(x[i].w - l.w));
+        if (++j == sv.n) break;
+        load_scores(j);
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int t = t0 + i * kFinishThreads + threadIdx.x;
+        if (t < sv.len) w[t] = sum[i];
+    }
+}
+
+// Behind the split kernel: blocks of (record stride, row) merge, the others add weights.
+__global__ void __launch_bounds__(kFinishThreads) chunk_finish_kernel(const FinishParams p) {
+    pdl_trigger();
+    pdl_wait();
+    if ((int)blockIdx.x >= p.merge_blocks) {
+        add_weights(p, blockIdx.x - p.merge_blocks);
+        return;
+    }
+    const int y = blockIdx.x % p.rows, lanes = p.merge_blocks / p.rows;
+    for (int i = blockIdx.x / p.rows; i < p.records; i += lanes) {
+        const Fragment f = read_record(p, i);
+        if (ragged_seq(p.rag, i / kNumKvHeads, nullptr).n == 0 || f.first >= f.last) continue;  // uniform
+        merge_row(p, f, y);
+        __syncthreads();  // before the next record's sums
+    }
+}
+
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Workspace of a call: the shares' records and partials, with weights the rows' lse, and in the split
 // form the scores.
 struct Layout {
     bool split;
-    int shares, rows;  // rows of a partial
+    int shares, rows, records;  // rows: of a partial
     size_t frags = 0, parts = 0, lse = 0, scores = 0, total = 0;
     int64_t score_stride = 0;
 };
-Layout layout(int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count) {
+Layout layout(int batch, int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count) {
     Layout l;
     l.split = max_q_len <= PGC_MAX_QUERIES;
     l.shares = l.split ? 2 * sm_count : sm_count / 2;
     l.rows = l.split ? max_q_len * kGroup : 2 * kBM;
-    l.parts = align256((size_t)l.shares * 2 * sizeof(Fragment));
+    l.records = l.split ? batch * kNumKvHeads : l.shares;
+    l.parts = align256((size_t)l.records * sizeof(Fragment));
     l.lse = align256(l.parts + (size_t)l.shares * 2 * l.rows * kPartial * sizeof(float));
     l.scores = align256(l.lse + (weights ? (size_t)total_q * kNumQHeads * sizeof(float) : 0));
     l.score_stride = (max_seq_len + kPage - 1) / kPage * kPage;
@@ -1218,8 +1421,8 @@ Layout layout(int total_q, int max_q_len, int max_seq_len, bool weights, int sm_
 
 }  // namespace
 
-size_t chunk_workspace_bytes(int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count) {
-    return layout(total_q, max_q_len, max_seq_len, weights, sm_count).total;
+size_t chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count) {
+    return layout(batch, total_q, max_q_len, max_seq_len, weights, sm_count).total;
 }
 
 cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtensorMap &tv, const uint16_t *v_pages,
@@ -1237,17 +1440,17 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) attr_set[dev] = true;
     }
-    const Layout lay = layout(rag.total_q, rag.max_q_len, rag.max_seq_len, weights != nullptr, sm_count);
+    const Layout lay = layout(rag.batch, rag.total_q, rag.max_q_len, rag.max_seq_len, weights != nullptr, sm_count);
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     if (lse == nullptr && weights != nullptr) lse = reinterpret_cast<float *>(ws + lay.lse);
-    MergeParams mp = {};
-    mp.rag = rag;
-    mp.frags = reinterpret_cast<const Fragment *>(ws + lay.frags);
-    mp.parts = reinterpret_cast<const float *>(ws + lay.parts);
-    mp.rows = lay.rows;
-    mp.gate = gate;
-    mp.out = out;
-    mp.lse = lse;
+    FinishParams fp = {};
+    fp.frags = reinterpret_cast<const Fragment *>(ws + lay.frags);
+    fp.parts = reinterpret_cast<const float *>(ws + lay.parts);
+    fp.records = lay.records;
+    fp.rows = lay.rows;
+    fp.gate = gate;
+    fp.out = out;
+    fp.lse = lse;
     if (lay.split) {
         SplitParams sp = {};
         sp.rag = rag;
@@ -1266,17 +1469,19 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
         const dim3 grid(lay.shares), block(kSplitThreads);
         cudaError_t e = weights != nullptr ? launch_pdl(chunk_split_kernel<true>, grid, block, kSplitSmem, stream, tk, tv, sp)
                                            : launch_pdl(chunk_split_kernel<false>, grid, block, kSplitSmem, stream, tk, tv, sp);
-        mp.tok = SplitTiling::kTok;
-        if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel<1>, dim3(lay.shares, lay.rows), dim3(256), 0, stream, mp);
-        if (e != cudaSuccess || weights == nullptr) return e;
-        AddParams ap = {};
-        ap.rag = rag;
-        ap.lse = lse;
-        ap.scores = sp.scores;
-        ap.score_stride = lay.score_stride;
-        ap.w = *weights;
-        return launch_pdl(chunk_add_kernel, dim3((rag.max_seq_len + kAddTokens - 1) / kAddTokens, kNumKvHeads, rag.batch),
-                          dim3(kAddThreads), 0, stream, ap);
+        if (e != cudaSuccess) return e;
+        fp.rag = rag;
+        // a few hundred blocks cover the records: most of a large batch's are of units not cut
+        fp.merge_blocks = (lay.records < lay.shares ? lay.records : lay.shares) * lay.rows;
+        int blocks = fp.merge_blocks;
+        if (weights != nullptr) {
+            fp.scores = sp.scores;
+            fp.score_stride = lay.score_stride;
+            fp.w = *weights;
+            fp.add_chunks = (rag.max_seq_len + kAddTokens - 1) / kAddTokens;
+            blocks += rag.batch * kNumKvHeads * fp.add_chunks;
+        }
+        return launch_pdl(chunk_finish_kernel, dim3(blocks), dim3(kFinishThreads), 0, stream, fp);
     }
     CUtensorMap tq;
     if (q_tensor_map(q, rag.total_q, &tq) != PGC_OK) return cudaErrorInvalidValue;
@@ -1293,8 +1498,7 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
     pp.parts = reinterpret_cast<float *>(ws + lay.parts);
     pp.scale_log2 = scale * kLog2e;
     cudaError_t e = launch_pdl(chunk_pair_kernel, dim3(2 * lay.shares), dim3(kPairThreads), PairSmem::kBytes, stream, tq, tk, tv, pp);
-    mp.tok = PairTiling::kTok;
-    if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel<8>, dim3(lay.shares, lay.rows / 8), dim3(256), 0, stream, mp);
+    if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel, dim3(lay.shares, lay.rows / kFinishWarps), dim3(kFinishThreads), 0, stream, fp);
     if (e != cudaSuccess || weights == nullptr) return e;
     return launch_chunk_weights(tq, tk, num_pages, block_tables, max_pages_per_seq, rag, scale, lse, *weights, sm_count, stream);
 }

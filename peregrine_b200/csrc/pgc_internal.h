@@ -132,7 +132,7 @@ struct ChunkWeights {
     int64_t stride, num_slots;
     const int32_t *slots;  // [batch], nullable
 };
-size_t chunk_workspace_bytes(int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count);
+size_t chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count);
 cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtensorMap &tv, const uint16_t *v_pages,
                          int64_t num_pages, const int32_t *block_tables, int max_pages_per_seq,
                          const RaggedBatch &rag, float scale, const uint16_t *gate, uint16_t *out, float *lse,
