@@ -583,8 +583,12 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         }
         const bool whole = w.t0 == 0 && w.t1 == w.tiles;
         float *part = p.parts + (int64_t)(index * 2 + (w.t0 > 0 ? 0 : 1)) * p.rag.max_q_len * kGroup * kPartial;
-        // dims d, d + 1 of row r
-        auto emit = [&](int r, int d, float2 acc) {
+        auto out_row = [&](int r) { return (int64_t)(w.row0 + r / kGroup) * kNumQHeads + w.kvh * kGroup + r % kGroup; };
+        // dims d, d + 1 of row r; loaded ahead of the barrier before their use
+        auto load_gate = [&](int r, int d) -> uint32_t {
+            return whole && p.gate != nullptr ? *reinterpret_cast<const uint32_t *>(p.gate + out_row(r) * kHeadDim + d) : 0;
+        };
+        auto emit = [&](int r, int d, float2 acc, uint32_t gv) {
             const float den = (l_s[r] + l_s[kRows + r]) + (l_s[2 * kRows + r] + l_s[3 * kRows + r]);
             const float ma = fmaxf(fmaxf(m_s[r], m_s[kRows + r]), fmaxf(m_s[2 * kRows + r], m_s[3 * kRows + r]));
             if (!whole) {
@@ -593,12 +597,11 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
                 if (d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(ma * kLn2, den);
                 return;
             }
-            const int64_t row = (int64_t)(w.row0 + r / kGroup) * kNumQHeads + w.kvh * kGroup + r % kGroup;
+            const int64_t row = out_row(r);
             const float inv = den == 0.f ? 0.f : 1.f / den;
             acc.x *= inv;
             acc.y *= inv;
             if (p.gate != nullptr) {
-                const uint32_t gv = *reinterpret_cast<const uint32_t *>(p.gate + row * kHeadDim + d);
                 acc.x = sigmoid_gate(acc.x, gv & 0xffffu);
                 acc.y = sigmoid_gate(acc.y, gv >> 16);
             }
@@ -621,14 +624,23 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
                 for (int i = 0; i < 32; ++i)
                     *reinterpret_cast<float2 *>(to + 8 * kJoinPitch + i * 8) = make_float2(o[i][2] * c1, o[i][3] * c1);
             }
-            sync();
-#pragma unroll 4
-            for (int r = 0; r < nrows; ++r) {
-                float2 acc = make_float2(0.f, 0.f);
+            uint32_t gv[kGroup];
 #pragma unroll
-                for (int q = 0; q < kConsumers; ++q)
-                    acc = __fadd2_rn(acc, *reinterpret_cast<const float2 *>(&buf[(q * jrows + r) * kJoinPitch + 2 * threadIdx.x]));
-                emit(r, 2 * threadIdx.x, acc);
+            for (int g = 0; g < kGroup; ++g) gv[g] = load_gate(g, 2 * threadIdx.x);
+            sync();
+            for (int rb = 0; rb < nrows; rb += kGroup) {
+#pragma unroll
+                for (int g = 0; g < kGroup; ++g) {
+                    float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int q = 0; q < kConsumers; ++q)
+                        acc = __fadd2_rn(acc, *reinterpret_cast<const float2 *>(&buf[(q * jrows + rb + g) * kJoinPitch + 2 * threadIdx.x]));
+                    emit(rb + g, 2 * threadIdx.x, acc, gv[g]);
+                }
+                if (rb + kGroup < nrows) {
+#pragma unroll
+                    for (int g = 0; g < kGroup; ++g) gv[g] = load_gate(rb + kGroup + g, 2 * threadIdx.x);
+                }
             }
             if (last) {
                 if (threadIdx.x == 0 && w.t0 == 0) write_record<SplitTiling>(&p.frags[w.seq * kNumKvHeads + w.kvh], w, *line, index);
@@ -652,7 +664,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
 #pragma unroll
                     for (int q = 0; q < kConsumers; ++q)
                         acc = __fadd2_rn(acc, *reinterpret_cast<const float2 *>(&join[(q * 16 + r) * (kJoinPitch / 4) + d]));
-                    emit(r, round * 64 + d, acc);
+                    emit(r, round * 64 + d, acc, load_gate(r, round * 64 + d));
                 }
                 sync();
             }
