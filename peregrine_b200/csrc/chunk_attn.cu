@@ -802,7 +802,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     tc_fence_before();
     cluster_sync_all();  // both CTAs' barriers are initialised before anyone signals them
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     auto leader_addr = [&](uint64_t *bar) { return cluster_map(smem_u32(bar), 0); };
     auto wait = [&](uint64_t *bar, uint32_t parity, int where) {
         return wait_or_abort(bar, parity, abort_flag, &g_chunk_err, where);
@@ -928,10 +928,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
     } else if (warp == kSoftmaxWarps) {
         // ------------------------------------------------------------ pair MMA issuer (leader)
-        if (leader && lane == 0) {
+        if (leader) {
+            const uint32_t me = elect_one();
             constexpr uint32_t idesc_s = umma_idesc(2 * kBM, kKeys, false, false);
             constexpr uint32_t idesc_o = umma_idesc(2 * kBM, kHeadDim, false, true);
-            const uint32_t q_addr = smem_u32(smem + PairSmem::kQ);
+            // descriptors step in units of 16 bytes; 128 KiB and more never carry out of the address field
+            const uint64_t q_desc = umma_desc(smem_u32(smem + PairSmem::kQ), 16, 1024);
+            const uint64_t k_desc = umma_desc(smem_u32(smem + PairSmem::kK), 16, 1024);
+            const uint64_t v_desc = umma_desc(smem_u32(smem + PairSmem::kV), kKeys * 128, 1024);
             // `ahead` is the next tile whose S is to be issued: S(g + 2) goes out behind PV(g), but
             // the first S of a unit only behind the last PV of the unit before it, because it waits
             // for that unit's Q to be replaced.
@@ -943,18 +947,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 if (at == a.t0 && !wait(q_full, aunit & 1, 4)) return false;
                 if (!wait(&k_full[sl], (ag / kKSlots) & 1, 5)) return false;
                 tc_fence_after();
-                const uint32_t k_addr = smem_u32(smem + PairSmem::kK + sl * kKHalf);
+                const uint64_t kd = k_desc + (uint32_t)(sl * (kKHalf >> 4));
 #pragma unroll
                 for (int kk = 0; kk < kHeadDim / 16; ++kk)
-                    umma2_ss(tmem + kTS + b * kKeys,
-                             umma_desc(q_addr + (kk >> 2) * (kBM * 128) + (kk & 3) * 32, 16, 1024),
-                             umma_desc(k_addr + (kk >> 2) * (64 * 128) + (kk & 3) * 32, 16, 1024),
-                             idesc_s, kk > 0 ? 1u : 0u);
-                umma2_commit_pair(&k_empty[sl]);
-                umma2_commit_pair(&s_full[b]);
+                    umma2_ss_elected(me, tmem + kTS + b * kKeys, q_desc + (((kk >> 2) * (kBM * 128) + (kk & 3) * 32) >> 4),
+                                     kd + (((kk >> 2) * (64 * 128) + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+                umma2_commit_pair_elected(me, &k_empty[sl]);
+                umma2_commit_pair_elected(me, &s_full[b]);
                 ++ag;
                 if (++at == a.t1) {
-                    umma2_commit_pair(q_empty);
+                    umma2_commit_pair_elected(me, q_empty);
                     more = walk_next<PairTiling>(p.rag, a);
                     at = a.t0;
                     ++aunit;
@@ -976,14 +978,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t v_addr = smem_u32(smem + PairSmem::kV + sl * kVHalf);
+                    const uint64_t vd = v_desc + (uint32_t)(sl * (kVHalf >> 4));
 #pragma unroll
                     for (int kk = 0; kk < kKeys / 16; ++kk)
-                        umma2_ts(tmem + kTO, tmem + kTS + b * kKeys + kk * 8,
-                                 umma_desc(v_addr + kk * 2048, kKeys * 128, 1024), idesc_o,
-                                 (t > w.t0 || kk > 0) ? 1u : 0u);
-                    umma2_commit_pair(&v_empty[sl]);
-                    umma2_commit_pair(&pv_done[b]);
+                        umma2_ts_elected(me, tmem + kTO, tmem + kTS + b * kKeys + kk * 8, vd + ((kk * 2048) >> 4), idesc_o,
+                                         (t > w.t0 || kk > 0) ? 1u : 0u);
+                    umma2_commit_pair_elected(me, &v_empty[sl]);
+                    umma2_commit_pair_elected(me, &pv_done[b]);
                 }
                 if (!ok || !walk_next<PairTiling>(p.rag, w)) break;
             }
