@@ -35,19 +35,24 @@ __device__ __forceinline__ float sigmoid_gate(float v, uint32_t gate_bits) {
 
 // =============================================================================================
 // The schedule. A unit is a (sequence, kv head, block of kTok query tokens); its tiles are blocks of
-// kKeys keys. The line of work is the units' tiles, units in that order.
+// kKeys keys. The line of work is the units' tiles, units in that order, each unit preceded by the
+// kOver tiles' worth of time that its start and end cost (Q's load, the pipeline's drain and the
+// epilogue), so that shares of many small units are not longer than shares of one large one.
 // =============================================================================================
 struct PairTiling {
     static constexpr int kTok = 64, kKeys = 128;
     static constexpr bool kWarpScan = false;
-    // A share below this many tiles costs more in its Q load, pipeline fill and partials than it saves.
-    static constexpr int kMinShare = 4;
+    static constexpr int kOver = 4;  // measured: 10 to 12 thousand cycles a unit, 2600 a tile
+    static constexpr int kMinShare = 8;
 };
 struct SplitTiling {
     static constexpr int kTok = PGC_MAX_QUERIES, kKeys = kPage;
     static constexpr bool kWarpScan = true;
-    static constexpr int kMinShare = 4;
+    static constexpr int kOver = 1;
+    static constexpr int kMinShare = 5;
 };
+static_assert(PairTiling::kMinShare > PairTiling::kOver && SplitTiling::kMinShare > SplitTiling::kOver,
+              "a share that begins in a unit's lead must reach its first tile");
 
 // Tiles of one unit: the keys that its last row sees, at least one tile (rows that see nothing still
 // get their zeros).
@@ -63,7 +68,8 @@ struct Walk {
     int row0, n, len;  // of the sequence
     int tiles;         // of the unit
     int t0, t1;        // the share's tiles of it
-    int left;          // tiles of the share from t0 on
+    int off;           // where the share enters the unit's kOver + tiles
+    int left;          // of the share from there on
 };
 
 __device__ __forceinline__ void walk_seq(const RaggedBatch &rag, Walk &w) {
@@ -73,16 +79,19 @@ __device__ __forceinline__ void walk_seq(const RaggedBatch &rag, Walk &w) {
     w.len = s.len;
 }
 template <class T>
-__device__ __forceinline__ void walk_unit(Walk &w, int t0) {
+__device__ __forceinline__ void walk_unit(Walk &w, int off) {
     w.tiles = unit_tiles<T>(w.n, w.len, w.qt);
-    w.t0 = t0;
-    w.t1 = w.tiles - t0 < w.left ? w.tiles : t0 + w.left;
+    w.off = off;
+    w.t0 = max(0, off - T::kOver);
+    const int cost = w.tiles + T::kOver;
+    w.t1 = w.left >= cost - off ? w.tiles : off + w.left - T::kOver;
 }
-// Next unit; false at the end of the share.
+// Next unit; false at the end of the share. A share that ends in a unit's lead leaves the unit to the
+// next share.
 template <class T>
 __device__ __forceinline__ bool walk_next(const RaggedBatch &rag, Walk &w) {
-    w.left -= w.t1 - w.t0;
-    if (w.left <= 0) return false;
+    w.left -= w.tiles + T::kOver - w.off;
+    if (w.left <= T::kOver) return false;
     if (++w.qt * T::kTok >= w.n) {
         w.qt = 0;
         if (++w.kvh == kNumKvHeads) {
@@ -95,6 +104,11 @@ __device__ __forceinline__ bool walk_next(const RaggedBatch &rag, Walk &w) {
     }
     walk_unit<T>(w, 0);
     return true;
+}
+// Whether the unit is the share's last: what walk_next would say, without stepping.
+template <class T>
+__device__ __forceinline__ bool walk_last(const Walk &w) {
+    return w.left - (w.tiles + T::kOver - w.off) <= T::kOver;
 }
 
 // The line's length and the shares it is cut into: the first `longer` ones take base + 1 tiles, the
@@ -126,24 +140,24 @@ __device__ __forceinline__ int share_of(const Line &l, int64_t tile) {
     return tile < cut ? (int)quotient(tile, l.base + 1) : l.longer + (int)quotient(tile - cut, l.base);
 }
 
-// Start of the walk: `off` tiles into sequence wk.seq, whose kv heads have `per` tiles each.
+// Start of the walk: `off` into sequence wk.seq, whose kv heads take `per` of the line each.
 template <class T>
 __device__ __forceinline__ void walk_start(Walk &wk, int64_t off, int64_t per, int64_t left) {
     wk.kvh = (int)quotient(off, per);
     off -= wk.kvh * per;
     for (wk.qt = 0;; ++wk.qt) {
-        const int t = unit_tiles<T>(wk.n, wk.len, wk.qt);
-        if (off < t) break;
-        off -= t;
+        const int c = unit_tiles<T>(wk.n, wk.len, wk.qt) + T::kOver;
+        if (off < c) break;
+        off -= c;
     }
     wk.left = (int)left;  // a grid of shares keeps it within int (PGC_CHUNK_MAX_ROWS)
     walk_unit<T>(wk, (int)off);
 }
 template <class T>
 __device__ __forceinline__ int64_t seq_cost(const RaggedSeq &s) {  // of one kv head
-    if (s.n <= T::kTok) return s.n == 0 ? 0 : unit_tiles<T>(s.n, s.len, 0);
+    if (s.n <= T::kTok) return s.n == 0 ? 0 : unit_tiles<T>(s.n, s.len, 0) + T::kOver;
     int64_t c = 0;
-    for (int qt = 0; qt * T::kTok < s.n; ++qt) c += unit_tiles<T>(s.n, s.len, qt);
+    for (int qt = 0; qt * T::kTok < s.n; ++qt) c += unit_tiles<T>(s.n, s.len, qt) + T::kOver;
     return c;
 }
 
@@ -159,7 +173,7 @@ __device__ __forceinline__ bool find_share(const RaggedBatch &rag, int64_t *cost
     const int lane = threadIdx.x & 31;
     wk.seq = -1;
     if (T::kWarpScan && rag.batch <= 32 * kChunks) {
-        // a sequence has at most 2^22 tiles (PGC_CHUNK_MAX_TOKENS), so 32 bits hold the line
+        // a sequence has at most 2^22 tiles and leads (PGC_CHUNK_MAX_TOKENS): 32 bits hold the line
         RaggedSeq s[kChunks];
         int c[kChunks], incl[kChunks], total = 0;
 #pragma unroll
@@ -252,7 +266,8 @@ struct Fragment {
 };
 template <class T>
 __device__ __forceinline__ void write_record(Fragment *f, const Walk &w, const Line &l, int index) {
-    const int last = w.t1 < w.tiles ? share_of(l, share_begin(l, index + 1) + (w.tiles - w.t1) - 1) : index;
+    const int behind = w.tiles + T::kOver - w.off - w.left;  // of the unit behind the share's end
+    const int last = w.t1 < w.tiles ? share_of(l, share_begin(l, index + 1) + behind - 1) : index;
     *reinterpret_cast<int4 *>(f) = make_int4(index, last, w.row0 + w.qt * T::kTok,
                                              min(T::kTok, w.n - w.qt * T::kTok) * kNumKvHeads + w.kvh);
 }
@@ -609,7 +624,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
             if (d == 0 && p.lse != nullptr) p.lse[row] = den == 0.f ? -INFINITY : ma * kLn2 + logf(den);
         };
         // the share's last unit: the ring and Q are free, and hold all rows at once
-        const bool last = w.left == w.t1 - w.t0;
+        const bool last = walk_last<SplitTiling>(w);
         if (nrows <= 4 || last) {
             // one round: [4 warps][4, 8 or 16 rows][256 dims]
             float *buf = nrows <= 4 ? join : reinterpret_cast<float *>(smem);
@@ -710,9 +725,15 @@ struct PairParams {
     uint16_t *out;
     float *lse;
     Fragment *frags;  // [pairs]
-    float *parts;     // [pairs][2][256][258]
+    float *parts;     // [pairs][2][kPairPart]
     float scale_log2;
 };
+
+// Floats of a pair's partial: O as [256 dims / 4][256 rows][4], then the rows' maxima and their sums, so
+// that the epilogue's threads, one per row, store 16 bytes side by side (a row of its own a thread took
+// 5 us a unit).
+constexpr int kPairStat = 2 * kBM * kHeadDim;
+constexpr int kPairPart = kPairStat + 2 * 2 * kBM;
 
 struct PairSmem {
     static constexpr int kQ = 0;
@@ -1086,39 +1107,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             tc_fence_after();
             const bool whole = w.t0 == 0 && w.t1 == w.tiles;
             const int slot = w.t0 > 0 ? 0 : 1;
+            const int64_t orow = (int64_t)(w.row0 + tok) * kNumQHeads + w.kvh * kGroup + r % kGroup;
+            uint32_t ow[32];  // the thread's 64 dims of a whole unit's row, bf16
             if (live) {
                 red[cg * kBM + r] = l;
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + qd) : "memory");
                 const float l_row = (red[r] + red[kBM + r]) + (red[2 * kBM + r] + red[3 * kBM + r]);
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + qd) : "memory");  // before the next unit's maxima
                 const float inv = l_row == 0.f ? 0.f : 1.f / l_row;
-                const int64_t orow = (int64_t)(w.row0 + tok) * kNumQHeads + w.kvh * kGroup + r % kGroup;
-                float *part = p.parts + ((int64_t)(pair * 2 + slot) * 2 * kBM + rank * kBM + r) * kPartial;
-                if (row_ok && cg == 0) {
+                float *part = p.parts + (int64_t)(pair * 2 + slot) * kPairPart + rank * kBM + r;
+                if (cg == 0) {
                     if (!whole) {
-                        part[0] = (m == -INFINITY) ? -INFINITY : m * kLn2;
-                        part[1] = l_row;
-                    } else if (p.lse != nullptr) {
+                        part[kPairStat] = (m == -INFINITY) ? -INFINITY : m * kLn2;
+                        part[kPairStat + 2 * kBM] = l_row;
+                    } else if (row_ok && p.lse != nullptr) {
                         p.lse[orow] = l_row == 0.f ? -INFINITY : m * kLn2 + logf(l_row);
                     }
                 }
-#pragma unroll 1
+#pragma unroll
                 for (int cc = 0; cc < 2; ++cc) {
                     float o[32];
                     const int col = cg * 64 + cc * 32;
                     tmem_ld32(tmem + lane_addr + kTO + col, o);
                     tmem_wait_ld();
-                    if (!row_ok) continue;
                     if (!whole) {
+                        // [dim / 4][row][4]: a warp's rows lie side by side
+                        float4 *dst = reinterpret_cast<float4 *>(p.parts + (int64_t)(pair * 2 + slot) * kPairPart) + rank * kBM + r;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2)
-                            *reinterpret_cast<float2 *>(part + 2 + col + i) = make_float2(o[i], o[i + 1]);
+                        for (int i = 0; i < 32; i += 4)
+                            dst[((col + i) / 4) * 2 * kBM] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                         continue;
                     }
                     // a row with nothing visible has P = 0 throughout: o = 0 and inv = 0
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] *= inv;
-                    if (p.gate != nullptr) {
+                    if (p.gate != nullptr && row_ok) {
                         const uint4 *gp = reinterpret_cast<const uint4 *>(p.gate + orow * kHeadDim + col);
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {
@@ -1129,24 +1152,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                                 o[i + k] = sigmoid_gate(o[i + k], (gw[k >> 1] >> ((k & 1) * 16)) & 0xffffu);
                         }
                     }
-                    uint16_t *dst = p.out + orow * kHeadDim + col;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        uint4 v;
-                        v.x = pack_bf16x2(o[i], o[i + 1]);
-                        v.y = pack_bf16x2(o[i + 2], o[i + 3]);
-                        v.z = pack_bf16x2(o[i + 4], o[i + 5]);
-                        v.w = pack_bf16x2(o[i + 6], o[i + 7]);
-                        *reinterpret_cast<uint4 *>(dst + i) = v;
-                    }
+                    for (int i = 0; i < 32; i += 2) ow[cc * 16 + i / 2] = pack_bf16x2(o[i], o[i + 1]);
                 }
             }
+            // O is read: the next unit's products may go on while this one's rows are stored
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(obar);
-            if (!walk_next<PairTiling>(p.rag, w)) break;
+            if (live && whole && row_ok) {
+                uint16_t *dst = p.out + orow * kHeadDim + cg * 64;
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                    *reinterpret_cast<uint4 *>(dst + 2 * i) = make_uint4(ow[i], ow[i + 1], ow[i + 2], ow[i + 3]);
+            }
+            if (walk_last<PairTiling>(w)) {
+                if (leader && threadIdx.x == 0 && w.t0 == 0) write_record<PairTiling>(&p.frags[pair], w, *line, pair);
+                break;
+            }
+            walk_next<PairTiling>(p.rag, w);
         }
-        if (leader && threadIdx.x == 0 && w.t0 == 0) write_record<PairTiling>(&p.frags[pair], w, *line, pair);
     }
     // neither CTA may leave (or free TMEM) while the pair MMA or the peer can still touch it
     tc_fence_before();
@@ -1167,7 +1192,7 @@ constexpr int kAddTokens = 2048;
 
 struct FinishParams {
     const Fragment *frags;
-    const float *parts;  // [shares][2][rows][258]
+    const float *parts;  // [shares][2][rows][258], the pair form's [pairs][2][kPairPart]
     int records;
     int rows;          // of a fragment
     int merge_blocks;  // the blocks behind them add weights
@@ -1191,54 +1216,77 @@ __device__ __forceinline__ int64_t fragment_at(const FinishParams &p, int i) {
     return (int64_t)(i == 0 ? 1 : 2 * i) * p.rows * kPartial;
 }
 
-// Behind the pair kernel: blocks (share, rows / 16), a warp per row; lane l owns dims [8 l, 8 l + 8).
+// Behind the pair kernel: block (share, y) joins rows [32 y, +32) of the unit that the share's end cuts.
+// Lane = row and a warp per 16 dims, as the partials lie; the joined rows go out through shared memory.
 __global__ void __launch_bounds__(kFinishThreads) chunk_merge_kernel(const FinishParams p) {
+    __shared__ float rows_s[32][kHeadDim + 1];
     pdl_trigger();
     pdl_wait();
     const Fragment f = read_record(p, blockIdx.x);
-    const int lane = threadIdx.x & 31;
-    const int r = blockIdx.y * kFinishWarps + (threadIdx.x >> 5);
-    const int kvh = f.rows_kvh % kNumKvHeads;
-    if (f.first >= f.last || r >= f.rows_kvh / kNumKvHeads * kGroup) return;
-    const float *base = p.parts + (int64_t)f.first * 2 * p.rows * kPartial + (int64_t)r * kPartial;
+    const int nrows = f.rows_kvh / kNumKvHeads * kGroup, kvh = f.rows_kvh % kNumKvHeads;
+    if (f.first >= f.last || (int)blockIdx.y * 32 >= nrows) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int r = blockIdx.y * 32 + lane;
     const int np = f.last - f.first + 1;
+    // fragment i: slot 1 of the first share, then slot 0 of the next ones
+    auto part = [&](int i) { return p.parts + (int64_t)((f.first + i) * 2 + (i == 0 ? 1 : 0)) * kPairPart; };
     float ma = -INFINITY, den = 0.f;
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    float4 acc[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
     for (int i = 0; i < np; ++i) {
-        const float *pc = base + fragment_at(p, i);
-        const float2 ml = *reinterpret_cast<const float2 *>(pc);
-        const float2 *o = reinterpret_cast<const float2 *>(pc + 2 + 8 * lane);
-        const float2 v[4] = {o[0], o[1], o[2], o[3]};
-        const float mx = fmaxf(ma, ml.x);
-        if (ml.x == -INFINITY) continue;  // the fragment saw nothing
-        const float corr = exp2f((ma - mx) * kLog2e), w = exp2f((ml.x - mx) * kLog2e);
+        const float *pc = part(i);
+        const float m = pc[kPairStat + r], l = pc[kPairStat + 2 * kBM + r];
+        const float4 *o = reinterpret_cast<const float4 *>(pc) + r;
+        const float4 v[4] = {o[(warp * 4) * 2 * kBM], o[(warp * 4 + 1) * 2 * kBM], o[(warp * 4 + 2) * 2 * kBM], o[(warp * 4 + 3) * 2 * kBM]};
+        if (m == -INFINITY) continue;  // the fragment saw nothing
+        const float mx = fmaxf(ma, m);
+        const float corr = exp2f((ma - mx) * kLog2e), w = exp2f((m - mx) * kLog2e);
         ma = mx;
-        den = den * corr + ml.y * w;
+        den = den * corr + l * w;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            acc[2 * k] = acc[2 * k] * corr + v[k].x * w;
-            acc[2 * k + 1] = acc[2 * k + 1] * corr + v[k].y * w;
+            acc[k].x = acc[k].x * corr + v[k].x * w;
+            acc[k].y = acc[k].y * corr + v[k].y * w;
+            acc[k].z = acc[k].z * corr + v[k].z * w;
+            acc[k].w = acc[k].w * corr + v[k].w * w;
         }
     }
-    const int64_t orow = (int64_t)(f.row + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup;
     const float inv = den == 0.f ? 0.f : 1.f / den;
-    float v[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = acc[k] * inv;
-    if (p.gate != nullptr) {
-        const uint4 gq = *reinterpret_cast<const uint4 *>(p.gate + orow * kHeadDim + 8 * lane);
-        const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = sigmoid_gate(v[k], (gw[k >> 1] >> ((k & 1) * 16)) & 0xffffu);
+    for (int k = 0; k < 4; ++k) {
+        float *to = &rows_s[lane][warp * 16 + 4 * k];
+        to[0] = acc[k].x * inv;
+        to[1] = acc[k].y * inv;
+        to[2] = acc[k].z * inv;
+        to[3] = acc[k].w * inv;
     }
-    uint4 q;
-    q.x = pack_bf16x2(v[0], v[1]);
-    q.y = pack_bf16x2(v[2], v[3]);
-    q.z = pack_bf16x2(v[4], v[5]);
-    q.w = pack_bf16x2(v[6], v[7]);
-    *reinterpret_cast<uint4 *>(p.out + orow * kHeadDim + 8 * lane) = q;
-    if (p.lse != nullptr && lane == 0) p.lse[orow] = (den == 0.f) ? -INFINITY : ma + logf(den);
+    if (warp == 0 && p.lse != nullptr && r < nrows)
+        p.lse[(int64_t)(f.row + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup] = (den == 0.f) ? -INFINITY : ma + logf(den);
+    __syncthreads();
+    // warp w: rows 2 w and 2 w + 1; lane l dims [8 l, 8 l + 8)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int rr = 2 * warp + q, row = blockIdx.y * 32 + rr;
+        if (row >= nrows) break;
+        const int64_t orow = (int64_t)(f.row + row / kGroup) * kNumQHeads + kvh * kGroup + row % kGroup;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = rows_s[rr][8 * lane + k];
+        if (p.gate != nullptr) {
+            const uint4 gq = *reinterpret_cast<const uint4 *>(p.gate + orow * kHeadDim + 8 * lane);
+            const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = sigmoid_gate(v[k], (gw[k >> 1] >> ((k & 1) * 16)) & 0xffffu);
+        }
+        uint4 o;
+        o.x = pack_bf16x2(v[0], v[1]);
+        o.y = pack_bf16x2(v[2], v[3]);
+        o.z = pack_bf16x2(v[4], v[5]);
+        o.w = pack_bf16x2(v[6], v[7]);
+        *reinterpret_cast<uint4 *>(p.out + orow * kHeadDim + 8 * lane) = o;
+    }
 }
 
 // One row of a cut unit behind the split kernel, by a block: the fragments (64 and more of a single long
@@ -1422,9 +1470,10 @@ Layout layout(int batch, int total_q, int max_q_len, int max_seq_len, bool weigh
     l.split = max_q_len <= PGC_MAX_QUERIES;
     l.shares = l.split ? 2 * sm_count : sm_count / 2;
     l.rows = l.split ? max_q_len * kGroup : 2 * kBM;
+    const size_t part = l.split ? (size_t)l.rows * kPartial : kPairPart;
     l.records = l.split ? batch * kNumKvHeads : l.shares;
     l.parts = align256((size_t)l.records * sizeof(Fragment));
-    l.lse = align256(l.parts + (size_t)l.shares * 2 * l.rows * kPartial * sizeof(float));
+    l.lse = align256(l.parts + (size_t)l.shares * 2 * part * sizeof(float));
     l.scores = align256(l.lse + (weights ? (size_t)total_q * kNumQHeads * sizeof(float) : 0));
     l.score_stride = (max_seq_len + kPage - 1) / kPage * kPage;
     l.total = l.scores;
@@ -1511,7 +1560,7 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
     pp.parts = reinterpret_cast<float *>(ws + lay.parts);
     pp.scale_log2 = scale * kLog2e;
     cudaError_t e = launch_pdl(chunk_pair_kernel, dim3(2 * lay.shares), dim3(kPairThreads), PairSmem::kBytes, stream, tq, tk, tv, pp);
-    if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel, dim3(lay.shares, lay.rows / kFinishWarps), dim3(kFinishThreads), 0, stream, fp);
+    if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel, dim3(lay.shares, lay.rows / 32), dim3(kFinishThreads), 0, stream, fp);
     if (e != cudaSuccess || weights == nullptr) return e;
     return launch_chunk_weights(tq, tk, num_pages, block_tables, max_pages_per_seq, rag, scale, lse, *weights, sm_count, stream);
 }
