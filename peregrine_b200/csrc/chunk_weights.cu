@@ -229,7 +229,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tc_fence_before();
     cluster_sync_all();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     auto leader_addr = [&](uint64_t *bar) { return cluster_map(smem_u32(bar), 0); };
     auto wait = [&](uint64_t *bar, uint32_t parity, int where) {
         return wait_or_abort(bar, parity, abort_flag, &g_cweights_err, where);
@@ -291,14 +291,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
     } else if (warp == kSumWarps) {
         // ------------------------------------------------------------ MMA issuer (leader)
-        if (leader && lane == 0) {
+        if (leader) {  // the whole warp, of which one lane acts (umma2_ss_elected)
+            const uint32_t me = elect_one();
             constexpr uint32_t idesc = umma_idesc(256, 256, false, false);
+            const uint64_t k_desc = umma_desc(smem_u32(smem + Smem::kK), 16, 1024);
+            const uint64_t q_desc = umma_desc(smem_u32(smem + Smem::kQ), 16, 1024);
             int g = 0, tile = 0;
             bool ok = true;
             for (int un = 0; ok; ++un) {
                 const int ks = un % kKSlots;
                 if (!wait(&k_full[ks], (un / kKSlots) & 1, 3)) break;
-                const uint32_t k_addr = smem_u32(smem + Smem::kK + ks * kKBytes);
+                const uint64_t kd = k_desc + (uint32_t)(ks * (kKBytes >> 4));
                 for (int qt = u.q0; ok && qt < u.q1; ++qt, ++tile) {
                     const int b = tile & 1;
                     if (tile >= 2 && !wait_or_abort_cluster(&d_empty[b], ((tile >> 1) - 1) & 1, abort_flag,
@@ -313,17 +316,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t q_addr = smem_u32(smem + Smem::kQ + sl * kQBytes);
+                        const uint64_t qd = q_desc + (uint32_t)(sl * (kQBytes >> 4));
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            umma2_ss(tmem + b * 256, umma_desc(k_addr + c * (128 * 128) + kk * 32, 16, 1024),
-                                     umma_desc(q_addr + kk * 32, 16, 1024), idesc, (c > 0 || kk > 0) ? 1u : 0u);
-                        umma2_commit_pair(&q_empty[sl]);
+                            umma2_ss_elected(me, tmem + b * 256, kd + ((c * (128 * 128) + kk * 32) >> 4), qd + ((kk * 32) >> 4),
+                                             idesc, (c > 0 || kk > 0) ? 1u : 0u);
+                        umma2_commit_pair_elected(me, &q_empty[sl]);
                     }
-                    if (ok) umma2_commit_pair(&d_full[b]);
+                    if (ok) umma2_commit_pair_elected(me, &d_full[b]);
                 }
                 if (!ok) break;
-                umma2_commit_pair(&k_empty[ks]);
+                umma2_commit_pair_elected(me, &k_empty[ks]);
                 if (!units_next(p.rag, u)) break;
             }
         }
