@@ -119,12 +119,12 @@ int pool_tensor_map(const void *pool, int64_t num_pages, CUtensorMap *out) {
     return PGC_OK;
 }
 
-int q_tensor_map(const void *q, int tokens, CUtensorMap *out) {
+int q_tensor_map(const void *q, int tokens, CUtensorMap *out, int box_tokens) {
     int dev = 0;
     int st = check_device(&dev);
     if (st != PGC_OK) return st;
     std::lock_guard<std::mutex> lk(g_mu);
-    MapKey key{dev, q, -(int64_t)tokens - 1};  // negative: distinct from pool keys
+    MapKey key{dev, q, -((int64_t)tokens * 64 + box_tokens) - 1};  // negative: distinct from pool keys
     auto it = g_maps.find(key);
     if (it != g_maps.end()) {
         *out = it->second;
@@ -137,7 +137,7 @@ int q_tensor_map(const void *q, int tokens, CUtensorMap *out) {
                                 (cuuint64_t)tokens};
     const cuuint64_t strides[2] = {(cuuint64_t)PGC_HEAD_DIM * 2,
                                    (cuuint64_t)PGC_HEAD_DIM * PGC_NUM_Q_HEADS * 2};
-    const cuuint32_t box[3] = {64, 4, 32};
+    const cuuint32_t box[3] = {64, 4, (cuuint32_t)box_tokens};
     const cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(q), dims, strides,
                     box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

@@ -1562,7 +1562,7 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
     cudaError_t e = launch_pdl(chunk_pair_kernel, dim3(2 * lay.shares), dim3(kPairThreads), PairSmem::kBytes, stream, tq, tk, tv, pp);
     if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel, dim3(lay.shares, lay.rows / 32), dim3(kFinishThreads), 0, stream, fp);
     if (e != cudaSuccess || weights == nullptr) return e;
-    return launch_chunk_weights(tq, tk, num_pages, block_tables, max_pages_per_seq, rag, scale, lse, *weights, sm_count, stream);
+    return launch_chunk_weights(q, tk, num_pages, block_tables, max_pages_per_seq, rag, scale, lse, *weights, sm_count, stream);
 }
 
 cudaError_t chunk_read_error(DevErrorHost *e, bool clear) {

@@ -5,12 +5,14 @@
 // The product is taken transposed, S^T = K Q^T: a key is then a TMEM lane, that is one thread, which
 // adds its row of exponentials in registers, with no exchange until the key's rows are all done. A
 // cluster of two CTAs (cta_group::2) owns 256 keys of one (sequence, kv head) at a time, 128 a CTA,
-// resident in shared memory, and streams the query rows past them in tiles of 64 tokens x 4 heads
-// (N = 256; each CTA stages half of them, in blocks of 64 dims). One pair adds all of a key's rows
+// resident in shared memory, and streams the query rows past them in tiles of 32 tokens x 4 heads
+// (N = 128; each CTA stages half of them, in blocks of 64 dims). One pair adds all of a key's rows
 // and is the only writer of its weight, so the sums' order is fixed and no atomics are needed.
-// TMEM holds two 256-column products: the exponentials of one overlap the MMAs of the next. Both
-// take 2048 cycles a tile at their peaks (16 exponentials a cycle and SM; 8192 bf16 FLOPs), so the
-// kernel is bound by both pipes together.
+// A tile takes 1024 cycles of the tensor pipe and as many of the MUFU pipe (16 exponentials a cycle
+// and SM), but three times that from its product to its sums, so TMEM holds four products, each with a
+// group of 4 warps of its own. The tensor pipe is 67 % busy on four prompts of 239 to 1600 tokens over
+// 4387 to 12000; moving a quarter or more of the exponentials to the FMA pipe (a polynomial) did not
+// raise that, two products of 256 columns instead of four of 128 lowered it by 5 %.
 // Units (sequence, kv head, 256 keys) are dealt to the pairs in consecutive shares of about equal
 // numbers of query tiles.
 #include <cuda.h>
@@ -27,14 +29,16 @@ PGC_DEFINE_ERROR_WORD(g_cweights_err);
 namespace {
 
 constexpr int kUnitKeys = 256;   // keys of a pair's unit, 128 a CTA
-constexpr int kTileTok = 64;     // query tokens of a tile (x 4 heads = 256 rows)
-constexpr int kSumWarps = 16;    // four per TMEM lane quarter, 64 columns each
-constexpr int kKWarps = 2;
-constexpr int kThreads = 32 * (kSumWarps + 1 + kKWarps + 1);
+constexpr int kTileTok = 32;     // query tokens of a tile (x 4 heads = 128 rows)
+constexpr int kCols = kTileTok * kGroup;
+constexpr int kBufs = 4;         // products in TMEM, each with a group of 4 warps (a key a thread)
+constexpr int kSumWarps = 4 * kBufs;
+constexpr int kLoadWarps = 2;    // TMA: one issuing warp delivers about 21 B a cycle to an SM, two 33
+constexpr int kThreads = 32 * (kSumWarps + 1 + kLoadWarps);
 constexpr int kKBytes = 128 * kHeadDim * 2;  // this CTA's keys: [4 dim blocks][128 rows][128 B]
-constexpr int kQBytes = 128 * 128;           // 128 query rows x 64 dims
+constexpr int kQBytes = 64 * 128;            // this CTA's 64 query rows x 64 dims
 constexpr int kKSlots = 2;
-constexpr int kQSlots = 5;
+constexpr int kQSlots = 10;
 constexpr uint32_t kTmemCols = 512;
 
 struct WeightsParams {
@@ -164,17 +168,18 @@ __device__ __forceinline__ bool find_units(const RaggedBatch &rag, int64_t *cost
 struct Smem {
     static constexpr int kK = 0;
     static constexpr int kQ = kK + kKSlots * kKBytes;
-    static constexpr int kLse = kQ + kQSlots * kQBytes;       // [2][256] fp32, log2 units
-    static constexpr int kSum = kLse + 2 * 256 * 4;           // [4 column quarters][128 keys] fp32
-    static constexpr int kBar = kSum + 4 * 128 * 4;
-    // leader: k_full[2], q_full[5], d_empty[2]; each: k_empty[2], q_empty[5], d_full[2]
-    static constexpr int kNumBars = 2 * (kKSlots + kQSlots + 2);
+    static constexpr int kLse = kQ + kQSlots * kQBytes;  // [groups][2][128] fp32, log2 units
+    static constexpr int kSum = kLse + kBufs * 2 * kCols * 4;  // [2][groups][128 keys] fp32
+    static constexpr int kBar = kSum + 2 * kBufs * 128 * 4;
+    // leader: k_full[2], q_full[10], d_empty[4]; each: k_empty[2], q_empty[10], d_full[4]
+    static constexpr int kNumBars = 2 * (kKSlots + kQSlots + kBufs);
     static constexpr int kUnits = kBar + kNumBars * 8;
     static constexpr int kTmemSlot = kUnits + 56;
     static constexpr int kAbort = kTmemSlot + 8;
     static constexpr int kBytes = kAbort + 8;
 };
 static_assert(sizeof(Units) <= 56 && Smem::kUnits % 8 == 0, "units slot");
+static_assert(kBufs * kCols <= (int)kTmemCols, "products");
 static_assert(Smem::kBytes <= 232448, "weights kernel shared memory exceeds the sm_100 limit");
 static_assert(PGC_CHUNK_MAX_BATCH * 8 <= kKSlots * kKBytes, "the schedule's scratch is the K buffers");
 
@@ -193,7 +198,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     uint64_t *k_full = reinterpret_cast<uint64_t *>(smem + Smem::kBar);  // leader: both CTAs' keys
     uint64_t *q_full = k_full + kKSlots;   // leader: both CTAs' query blocks
     uint64_t *d_empty = q_full + kQSlots;  // leader: both CTAs' sum warps have read the product
-    uint64_t *k_empty = d_empty + 2;
+    uint64_t *k_empty = d_empty + kBufs;
     uint64_t *q_empty = k_empty + kKSlots;
     uint64_t *d_full = q_empty + kQSlots;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Smem::kTmemSlot);
@@ -206,16 +211,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < kKSlots; ++s) {
-            mbar_init(&k_full[s], 2 * kKWarps);
+            mbar_init(&k_full[s], 2 * kLoadWarps);
             mbar_init(&k_empty[s], 1);
         }
         for (int s = 0; s < kQSlots; ++s) {
             mbar_init(&q_full[s], 2);
             mbar_init(&q_empty[s], 1);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < kBufs; ++b) {
             mbar_init(&d_full[b], 1);
-            mbar_init(&d_empty[b], 2 * kSumWarps);
+            mbar_init(&d_empty[b], 8);  // a group of each CTA
         }
         fence_mbar_init();
     }
@@ -236,46 +241,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     };
     Units u = *share;
 
-    if (warp > kSumWarps && warp <= kSumWarps + kKWarps) {
-        // ------------------------------------------------------------ TMA: keys, 4 pages a warp
-        const int kw = warp - kSumWarps - 1;
+    if (warp > kSumWarps) {
+        // ------------------------------------------------------------ TMA: keys and query rows
+        // Warp lw loads 4 of this CTA's 8 pages of each unit's keys and every second 64-dim block of the
+        // query rows. The next unit's keys go out behind the first tiles of this unit: their buffer is
+        // free when the unit before this one is done.
+        const int lw = warp - kSumWarps - 1;
         if (lane == 0) {
             const uint64_t pol = l2_policy_evict_first();
-            if (kw == 0) tma_prefetch_desc(&tmk);
-            for (int un = 0;; ++un) {
+            tma_prefetch_desc(lw == 0 ? &tmk : &tmq);
+            auto load_keys = [&](const Units &v, int un) -> bool {
                 const int sl = un % kKSlots;
-                if (un >= kKSlots && !wait(&k_empty[sl], ((un / kKSlots) - 1) & 1, 1)) break;
-                const int key0 = u.kt * kUnitKeys + (int)rank * 128;
+                if (un >= kKSlots && !wait(&k_empty[sl], ((un / kKSlots) - 1) & 1, 1)) return false;
+                const int key0 = v.kt * kUnitKeys + (int)rank * 128;
                 int npg = 0;
-                for (int pp = 4 * kw; pp < 4 * kw + 4; ++pp)
-                    if (key0 + pp * kPage < u.len) ++npg;
+                for (int pp = 4 * lw; pp < 4 * lw + 4; ++pp)
+                    if (key0 + pp * kPage < v.len) ++npg;
                 const uint32_t kbar = leader_addr(&k_full[sl]);
                 mbar_arrive_expect_tx_cluster(kbar, (uint32_t)npg * 4 * 2048);
                 uint8_t *dst = smem + Smem::kK + sl * kKBytes;
-                for (int pp = 4 * kw; pp < 4 * kw + npg; ++pp) {
-                    int page = p.block_tables[(int64_t)u.seq * p.max_pages_per_seq + (key0 >> 4) + pp];
+                for (int pp = 4 * lw; pp < 4 * lw + npg; ++pp) {
+                    int page = p.block_tables[(int64_t)v.seq * p.max_pages_per_seq + (key0 >> 4) + pp];
                     if (page < 0 || page >= p.num_pages) {
                         record_error(&g_cweights_err, kErrPageOutOfRange, page);
                         page = 0;
                     }
-                    const int row = (page * kNumKvHeads + u.kvh) * kPage;
+                    const int row = (page * kNumKvHeads + v.kvh) * kPage;
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
                         tma_load_2d_pair(dst + c * (128 * 128) + pp * 2048, &tmk, c * 64, row, kbar, pol);
                 }
-                if (!units_next(p.rag, u)) break;
-            }
-        }
-    } else if (warp > kSumWarps + kKWarps) {
-        // ------------------------------------------------------------ TMA: query rows, 64-dim blocks
-        if (lane == 0) {
-            tma_prefetch_desc(&tmq);
-            int g = 0;
-            bool ok = true;
-            while (ok) {
+                return true;
+            };
+            constexpr int kLead = 2;  // tiles of a unit that go out before the next unit's keys
+            int g = lw;               // this warp's query blocks: g, g + 2, ...
+            bool ok = load_keys(u, 0);
+            for (int un = 0; ok; ++un) {
+                Units nu = u;
+                const bool more = units_next(p.rag, nu);
                 for (int qt = u.q0; ok && qt < u.q1; ++qt) {
-                    const int tok = u.row0 + qt * kTileTok + (int)rank * 32;
-                    for (int c = 0; c < 4; ++c, ++g) {
+                    if (qt == u.q0 + kLead && more) ok = load_keys(nu, un + 1);
+                    const int tok = u.row0 + qt * kTileTok + (int)rank * (kTileTok / 2);
+                    for (int c = lw; ok && c < 4; c += 2, g += 2) {
                         const int sl = g % kQSlots;
                         if (g >= kQSlots && !wait(&q_empty[sl], ((g / kQSlots) - 1) & 1, 2)) {
                             ok = false;
@@ -286,14 +293,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         tma_load_3d_pair(smem + Smem::kQ + sl * kQBytes, &tmq, c * 64, u.kvh * kGroup, tok, qbar);
                     }
                 }
-                if (!ok || !units_next(p.rag, u)) break;
+                if (!ok || !more) break;
+                if (u.q1 - u.q0 <= kLead) ok = load_keys(nu, un + 1);
+                u = nu;
             }
         }
     } else if (warp == kSumWarps) {
         // ------------------------------------------------------------ MMA issuer (leader)
         if (leader) {  // the whole warp, of which one lane acts (umma2_ss_elected)
             const uint32_t me = elect_one();
-            constexpr uint32_t idesc = umma_idesc(256, 256, false, false);
+            constexpr uint32_t idesc = umma_idesc(256, kCols, false, false);
             const uint64_t k_desc = umma_desc(smem_u32(smem + Smem::kK), 16, 1024);
             const uint64_t q_desc = umma_desc(smem_u32(smem + Smem::kQ), 16, 1024);
             int g = 0, tile = 0;
@@ -303,9 +312,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (!wait(&k_full[ks], (un / kKSlots) & 1, 3)) break;
                 const uint64_t kd = k_desc + (uint32_t)(ks * (kKBytes >> 4));
                 for (int qt = u.q0; ok && qt < u.q1; ++qt, ++tile) {
-                    const int b = tile & 1;
-                    if (tile >= 2 && !wait_or_abort_cluster(&d_empty[b], ((tile >> 1) - 1) & 1, abort_flag,
-                                                            &g_cweights_err, 4)) {
+                    const int b = tile % kBufs;
+                    if (tile >= kBufs && !wait_or_abort_cluster(&d_empty[b], ((tile / kBufs) - 1) & 1, abort_flag,
+                                                                &g_cweights_err, 4)) {
                         ok = false;
                         break;
                     }
@@ -319,7 +328,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         const uint64_t qd = q_desc + (uint32_t)(sl * (kQBytes >> 4));
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            umma2_ss_elected(me, tmem + b * 256, kd + ((c * (128 * 128) + kk * 32) >> 4), qd + ((kk * 32) >> 4),
+                            umma2_ss_elected(me, tmem + b * kCols, kd + ((c * (128 * 128) + kk * 32) >> 4), qd + ((kk * 32) >> 4),
                                              idesc, (c > 0 || kk > 0) ? 1u : 0u);
                         umma2_commit_pair_elected(me, &q_empty[sl]);
                     }
@@ -332,89 +341,99 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
     } else {
         // ------------------------------------------------------------ exponentials and their sums
-        // Warp (qd, cg): keys 32 qd + lane of this CTA, columns [64 cg, +64) of a tile. A wait that
-        // gives up does not take a warp out of step with the named barriers (see chunk_attn.cu).
-        const int qd = warp & 3, cg = warp >> 2;
-        const uint32_t lane_addr = (uint32_t)(qd * 32) << 16;
-        float *lse_s = reinterpret_cast<float *>(smem + Smem::kLse);
+        // Group `grp` takes the products of its buffer, every fourth tile; its warp qd the keys
+        // 32 qd + lane of this CTA. A wait that gives up does not take a warp out of step with the named
+        // barriers (see chunk_attn.cu).
+        const int grp = warp >> 2, qd = warp & 3;
+        const int gtid = threadIdx.x & 127;
+        const uint32_t src = tmem + ((uint32_t)(qd * 32) << 16) + grp * kCols;
+        float *lse_s = reinterpret_cast<float *>(smem + Smem::kLse) + grp * 2 * kCols;
         float *sum_s = reinterpret_cast<float *>(smem + Smem::kSum);
-        const uint32_t ebar[2] = {leader_addr(&d_empty[0]), leader_addr(&d_empty[1])};
+        const uint32_t ebar = leader_addr(&d_empty[grp]);
         const float c = p.scale_log2;
-        // Column threadIdx.x's lse in log2 units; +inf for a row that sees nothing or is not the
-        // sequence's, whose exponentials are then 0 or masked.
-        auto load_lse = [&](const Units &v, int qt) -> float {
-            const int tok = qt * kTileTok + (int)threadIdx.x / kGroup;
-            if (threadIdx.x >= 256 || tok >= v.n) return INFINITY;
-            const float x = p.lse[(int64_t)(v.row0 + tok) * kNumQHeads + v.kvh * kGroup + threadIdx.x % kGroup];
+        // Column gtid's lse in log2 units; +inf for a row whose sum is 0, so that its -inf scores add
+        // nothing, and for the rows that are not the sequence's.
+        auto load_lse = [&](int qt) -> float {
+            const int tok = qt * kTileTok + gtid / kGroup;
+            if (tok >= u.n) return INFINITY;
+            const float x = p.lse[(int64_t)(u.row0 + tok) * kNumQHeads + u.kvh * kGroup + gtid % kGroup];
             return x == -INFINITY ? INFINITY : x * kLog2e;
         };
-        int tile = 0, slot_seq = -1;
+        int tile = 0, slot_seq = -1;  // tile: the share's tiles before this unit
         int64_t slot = -1;
-        if (threadIdx.x < 256) lse_s[threadIdx.x] = load_lse(u, u.q0);
-        asm volatile("bar.sync 1, %0;" ::"r"(kSumWarps * 32) : "memory");
-        for (bool more = true; more;) {
+        for (int un = 0;; ++un) {
             if (u.seq != slot_seq) {
                 slot_seq = u.seq;
                 slot = ragged_slot(p.w.slots, p.w.num_slots, u.seq, &g_cweights_err);
             }
-            Units nu = u;
-            more = units_next(p.rag, nu);
             const int key = u.kt * kUnitKeys + (int)rank * 128 + qd * 32 + lane;
             const int P = u.len - u.n;
             float2 sum2 = make_float2(0.f, 0.f);
-            for (int qt = u.q0; qt < u.q1; ++qt, ++tile) {
-                const int b = tile & 1;
-                // the next tile's lse, in flight while this one is summed
-                const bool last = qt + 1 == u.q1;
-                const float next = last ? (more ? load_lse(nu, nu.q0) : 0.f) : load_lse(u, qt + 1);
-                wait(&d_full[b], (tile >> 1) & 1, 6);
+            const int first = u.q0 + ((grp - tile) & (kBufs - 1));  // this group's first tile of the unit
+            int buf = 0;
+            if (first < u.q1) {
+                lse_s[gtid] = load_lse(first);
+                asm volatile("bar.sync %0, 128;" ::"r"(2 + grp) : "memory");
+            }
+            for (int qt = first; qt < u.q1; qt += kBufs) {
+                const int g = tile + qt - u.q0;  // of the share
+                // the group's next tile's lse, in flight while this one is summed
+                const float next = qt + kBufs < u.q1 ? load_lse(qt + kBufs) : 0.f;
+                wait(&d_full[grp], (g / kBufs) & 1, 6);
                 tc_fence_after();
-                const float *ls = lse_s + b * 256;
-                const int hi = min(kTileTok, u.n - qt * kTileTok) * kGroup;   // the sequence's columns
-                const int lo = (key - P - qt * kTileTok) * kGroup;            // the first that sees this key
+                const float *ls = lse_s + buf * kCols;
+                const int hi = min(kTileTok, u.n - qt * kTileTok) * kGroup;  // the sequence's columns
+                const int lo = (key - P - qt * kTileTok) * kGroup;           // the first that sees this key
                 const int lo_warp = (key - lane + 31 - P - qt * kTileTok) * kGroup;
+                float sv[2][32];  // the next 32 columns are read while these are summed
+                tmem_ld32(src, sv[0]);
+                tmem_wait_ld();
 #pragma unroll
-                for (int cc = 0; cc < 2; ++cc) {
-                    const int col = cg * 64 + cc * 32;
+                for (int k = 0; k < kCols / 32; ++k) {
+                    const int col = k * 32;
                     if (col >= hi) break;
-                    float sv[32];
-                    tmem_ld32(tmem + lane_addr + b * 256 + col, sv);
-                    tmem_wait_ld();
+                    if (k + 1 < kCols / 32) tmem_ld32(src + col + 32, sv[(k + 1) & 1]);
+                    float(&v)[32] = sv[k & 1];
                     if (lo_warp <= col && col + 32 <= hi) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
                             const float4 l4 = *reinterpret_cast<const float4 *>(ls + col + i);
-                            const float2 x = __ffma2_rn(make_float2(sv[i], sv[i + 1]), make_float2(c, c),
-                                                        make_float2(-l4.x, -l4.y));
-                            const float2 y = __ffma2_rn(make_float2(sv[i + 2], sv[i + 3]), make_float2(c, c),
-                                                        make_float2(-l4.z, -l4.w));
+                            const float2 x = __ffma2_rn(make_float2(v[i], v[i + 1]), make_float2(c, c), make_float2(-l4.x, -l4.y));
+                            const float2 y = __ffma2_rn(make_float2(v[i + 2], v[i + 3]), make_float2(c, c), make_float2(-l4.z, -l4.w));
                             sum2 = __fadd2_rn(sum2, make_float2(fast_exp2(x.x), fast_exp2(x.y)));
                             sum2 = __fadd2_rn(sum2, make_float2(fast_exp2(y.x), fast_exp2(y.y)));
                         }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
-                            const float e = fast_exp2(sv[i] * c - ls[col + i]);
+                            const float e = fast_exp2(v[i] * c - ls[col + i]);
                             if (col + i >= lo && col + i < hi) sum2.x += e;
                         }
                     }
+                    tmem_wait_ld();
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(ebar[b]);
-                if (threadIdx.x < 256) lse_s[(b ^ 1) * 256 + threadIdx.x] = next;
-                // the next tile's lse is in place, and this tile's may be replaced
-                asm volatile("bar.sync 1, %0;" ::"r"(kSumWarps * 32) : "memory");
+                if (lane == 0) mbar_arrive_cluster(ebar);
+                buf ^= 1;
+                if (qt + kBufs < u.q1) {
+                    // one barrier a tile: a buffer is written again two tiles on, when all have read it
+                    lse_s[buf * kCols + gtid] = next;
+                    asm volatile("bar.sync %0, 128;" ::"r"(2 + grp) : "memory");
+                }
             }
-            sum_s[cg * 128 + qd * 32 + lane] = sum2.x + sum2.y;
+            // Join: double-buffered by unit, so one barrier also keeps the next writes off these reads
+            // and the next unit's lse off this one's.
+            float *mine = sum_s + (un & 1) * kBufs * 128;
+            mine[grp * 128 + qd * 32 + lane] = sum2.x + sum2.y;
             asm volatile("bar.sync 1, %0;" ::"r"(kSumWarps * 32) : "memory");
-            if (cg == 0 && slot >= 0 && key < u.len) {
+            if (warp < 4 && slot >= 0 && key < u.len) {
                 const int k = qd * 32 + lane;
                 p.w.weights[(slot * kNumKvHeads + u.kvh) * p.w.stride + key] +=
-                    (sum_s[k] + sum_s[128 + k]) + (sum_s[256 + k] + sum_s[384 + k]);
+                    (mine[k] + mine[128 + k]) + (mine[256 + k] + mine[384 + k]);
             }
-            // the sums are read before the next unit's tiles end: the tile barrier orders them
-            u = nu;
+            tile += u.q1 - u.q0;
+            if (!units_next(p.rag, u)) break;
         }
     }
     tc_fence_before();
@@ -427,7 +446,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 }  // namespace
 
-cudaError_t launch_chunk_weights(const CUtensorMap &tq, const CUtensorMap &tk, int64_t num_pages,
+cudaError_t launch_chunk_weights(const uint16_t *q, const CUtensorMap &tk, int64_t num_pages,
                                  const int32_t *block_tables, int max_pages_per_seq, const RaggedBatch &rag,
                                  float scale, const float *lse, const ChunkWeights &weights, int sm_count,
                                  cudaStream_t stream) {
@@ -440,6 +459,8 @@ cudaError_t launch_chunk_weights(const CUtensorMap &tq, const CUtensorMap &tk, i
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) attr_set[dev] = true;
     }
+    CUtensorMap tq;
+    if (q_tensor_map(q, rag.total_q, &tq, kTileTok / 2) != PGC_OK) return cudaErrorInvalidValue;
     WeightsParams wp = {};
     wp.rag = rag;
     wp.block_tables = block_tables;

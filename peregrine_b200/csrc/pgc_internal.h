@@ -24,8 +24,8 @@ struct DevErrorHost {
 int pool_tensor_map(const void *pool, int64_t num_pages, CUtensorMap *out);
 int current_sm_count();
 // Tensor map over a chunk's queries [tokens][16][256] bf16 viewed as (dim, head, token),
-// 64 x 4 x 32 boxes, 128-byte swizzle. Cached per (device, pointer, tokens).
-int q_tensor_map(const void *q, int tokens, CUtensorMap *out);
+// 64 x 4 x box_tokens (16 or 32) boxes, 128-byte swizzle. Cached per (device, pointer, tokens, box).
+int q_tensor_map(const void *q, int tokens, CUtensorMap *out, int box_tokens = 32);
 int tiled_map_2d(const void *ptr, int elem_bytes, int64_t inner, int64_t outer, int box_inner,
                  int box_outer, bool swizzle128, CUtensorMap *out);
 
@@ -140,7 +140,7 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
 cudaError_t chunk_read_error(DevErrorHost *e, bool clear);
 
 // chunk_weights.cu: weights += column sums of exp(scale q.k - lse) over the batch's rows
-cudaError_t launch_chunk_weights(const CUtensorMap &tq, const CUtensorMap &tk, int64_t num_pages,
+cudaError_t launch_chunk_weights(const uint16_t *q, const CUtensorMap &tk, int64_t num_pages,
                                  const int32_t *block_tables, int max_pages_per_seq, const RaggedBatch &rag,
                                  float scale, const float *lse, const ChunkWeights &weights, int sm_count,
                                  cudaStream_t stream);
