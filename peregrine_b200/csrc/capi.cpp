@@ -119,6 +119,35 @@ int pool_tensor_map(const void *pool, int64_t num_pages, CUtensorMap *out) {
     return PGC_OK;
 }
 
+int pool_page_map(const void *pool, int64_t num_pages, CUtensorMap *out) {
+    int dev = 0;
+    int st = check_device(&dev);
+    if (st != PGC_OK) return st;
+    std::lock_guard<std::mutex> lk(g_mu);
+    static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
+    MapKey key{dev, pool, num_pages};
+    auto it = cache.find(key);
+    if (it != cache.end()) {
+        *out = it->second;
+        return PGC_OK;
+    }
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return PGC_ERR_CUDA;
+    CUtensorMap m;
+    const cuuint64_t dims[3] = {64, (cuuint64_t)num_pages * 4 * 16, 4};
+    const cuuint64_t strides[2] = {(cuuint64_t)PGC_HEAD_DIM * 2, 128};
+    const cuuint32_t box[3] = {64, 16, 4};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(pool), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return PGC_ERR_CUDA;
+    if (cache.size() > 4096) cache.clear();
+    cache.emplace(key, m);
+    *out = m;
+    return PGC_OK;
+}
+
 int q_tensor_map(const void *q, int tokens, CUtensorMap *out, int box_tokens) {
     int dev = 0;
     int st = check_device(&dev);
@@ -494,8 +523,10 @@ static int chunk_call(const uint16_t *q, const uint16_t *k_pages, const uint16_t
     int st = check_device(nullptr);
     if (st != PGC_OK) return st;
     CUtensorMap tk, tv;
-    if ((st = pool_tensor_map(k_pages, num_pages, &tk)) != PGC_OK) return st;
-    if ((st = pool_tensor_map(v_pages, num_pages, &tv)) != PGC_OK) return st;
+    // the split form loads a page's head in one box, the pair form in boxes of 64 dims
+    const auto map = max_q_len <= PGC_MAX_QUERIES ? pool_page_map : pool_tensor_map;
+    if ((st = map(k_pages, num_pages, &tk)) != PGC_OK) return st;
+    if ((st = map(v_pages, num_pages, &tv)) != PGC_OK) return st;
     RaggedBatch rag;
     rag.q_starts = q_starts;
     rag.seq_lens = seq_lens;

@@ -329,6 +329,15 @@ __device__ __forceinline__ void bulk_load(void *smem_dst, const void *src, uint3
                  : "memory");
 }
 
+// One (page, kv head) of a pool, by its pool_page_map.
+__device__ __forceinline__ void tma_load_page(void *smem_dst, const void *tmap, int32_t row, uint64_t *bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%2, %3, %2}], [%4], %5;" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(0), "r"(row), "r"(smem_u32(bar)), "l"(policy)
+        : "memory");
+}
+
 template <bool kScores>
 __global__ void __launch_bounds__(kSplitThreads, 2)
     chunk_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
@@ -411,11 +420,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
                         uint8_t *stage = smem + SplitSmem::kRing + s * kStageBytes;
                         mbar_arrive_expect_tx(&full[s], kStageBytes);
                         const int row = (page * kNumKvHeads + w.kvh) * kPage;
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) tma_load_2d(stage + c * 2048, &tmk, c * 64, row, &full[s], pol);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            tma_load_2d(stage + kTileBytes + c * 2048, &tmv, c * 64, row, &full[s], pol);
+                        tma_load_page(stage, &tmk, row, &full[s], pol);
+                        tma_load_page(stage + kTileBytes, &tmv, row, &full[s], pol);
                     } else {
                         mbar_arrive(&full[s]);  // an empty cache: the tile is all masked
                     }

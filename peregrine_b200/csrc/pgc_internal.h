@@ -22,6 +22,9 @@ struct DevErrorHost {
 // Tensor map over one paged pool viewed as [num_pages * 4 * 16 rows][256] bf16, 64 x 16 boxes,
 // 128-byte swizzle. Cached per (device, base pointer, num_pages).
 int pool_tensor_map(const void *pool, int64_t num_pages, CUtensorMap *out);
+// The same pool as [4 blocks of 64 dims][rows][64], 4 x 16 x 64 boxes: one page's kv head a box, laid
+// out in shared memory as four boxes of the map above.
+int pool_page_map(const void *pool, int64_t num_pages, CUtensorMap *out);
 int current_sm_count();
 // Tensor map over a chunk's queries [tokens][16][256] bf16 viewed as (dim, head, token),
 // 64 x 4 x box_tokens (16 or 32) boxes, 128-byte swizzle. Cached per (device, pointer, tokens, box).
