@@ -313,8 +313,8 @@ struct SplitSmem {
     static constexpr int kM = kJoin + kConsumers * 4 * kJoinPitch * 4;  // [4 warps][16 rows]
     static constexpr int kL = kM + kConsumers * kRows * 4;
     static constexpr int kBar = kL + kConsumers * kRows * 4;  // full[4], empty[4], q_full[2], q_empty[2]
-    static constexpr int kWalk = kBar + (2 * kStages + 4) * 8;
-    static constexpr int kLine = kWalk + 48;
+    static constexpr int kWalk = kBar + (2 * kStages + 4) * 8;  // per consumer warp
+    static constexpr int kLine = kWalk + kConsumers * sizeof(Walk);
     static constexpr int kBytes = kLine + 24;
 };
 constexpr int kSplitSmem = SplitSmem::kBytes + 1024;  // + alignment slack
@@ -447,9 +447,14 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     const int v_dim_off = (mi >> 1) * 8;
     auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(kConsumers * 32) : "memory"); };
 
+    // The walk lives in shared memory, a copy per warp: the tile loop needs the registers.
+    Walk *const ws = reinterpret_cast<Walk *>(smem + SplitSmem::kWalk) + warp;
+    if (lane == 0) *ws = w;
+    __syncwarp();
     int g0 = 0;  // the CTA's tiles before this unit
     for (int unit = 0;; ++unit) {
-        const int n = w.n, L = w.len, nrows = n * kGroup, qb = unit & 1;
+        const int n = ws->n, L = ws->len, nrows = n * kGroup, qb = unit & 1, t1 = ws->t1;
+        g0 -= ws->t0;  // tile t is the CTA's g0 + t
         // visible token bound per C row: row j sees tokens < L - n + j + 1; rows of nobody see none
         const int vis0 = r0 < nrows ? L - n + r0 / kGroup + 1 : 0;
         const int vis1 = r0 + 8 < nrows ? L - n + (r0 + 8) / kGroup + 1 : 0;
@@ -461,9 +466,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         // A wait that gives up is recorded and the warp runs on (every later wait is bounded too), so
         // that the four warps stay in step at their barriers.
         if (!mbar_wait_bounded(&q_full[qb], (unit >> 1) & 1)) record_error(&g_chunk_err, kErrWaitTimeout, 23);
-        int t = w.t0 + ((warp - g0) & (kConsumers - 1));  // this warp's first tile: (g0 + t - t0) % 4 == warp
-        for (; t < w.t1; t += kConsumers) {
-            const int g = g0 + t - w.t0;
+        for (int t = ws->t0 + ((warp - g0 - ws->t0) & (kConsumers - 1)); t < t1; t += kConsumers) {
+            const int g = g0 + t;  // g % 4 == warp
             const int s = g % kStages;
             if (!mbar_wait_bounded(&full[s], (g / kStages) & 1)) {
                 record_error(&g_chunk_err, kErrWaitTimeout, 24);
@@ -503,7 +507,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
             }
             if (kScores) {
                 // the rows and lanes of a tile fill whole 32-byte sectors of [token][head]
-                float *s0 = p.scores + (((int64_t)(w.row0 + r0 / kGroup) * kNumKvHeads + w.kvh) * p.score_stride + tok0 + cpair) * kGroup + r0 % kGroup;
+                float *s0 = p.scores + (((int64_t)(ws->row0 + r0 / kGroup) * kNumKvHeads + ws->kvh) * p.score_stride + tok0 + cpair) * kGroup + r0 % kGroup;
                 float *s1 = s0 + 2 * kNumKvHeads * p.score_stride * kGroup;  // row r0 + 8: two query tokens on
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -602,6 +606,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
             l_s[warp * kRows + r0] = l0 * c0;
             l_s[warp * kRows + r0 + 8] = l1 * c1;
         }
+        Walk w = *ws;
         const bool whole = w.t0 == 0 && w.t1 == w.tiles;
         float *part = p.parts + (int64_t)(index * 2 + (w.t0 > 0 ? 0 : 1)) * p.rag.max_q_len * kGroup * kPartial;
         auto out_row = [&](int r) { return (int64_t)(w.row0 + r / kGroup) * kNumQHeads + w.kvh * kGroup + r % kGroup; };
@@ -691,8 +696,11 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
             }
         }
         if (threadIdx.x == 0 && w.t0 == 0) write_record<SplitTiling>(&p.frags[w.seq * kNumKvHeads + w.kvh], w, *line, index);
-        g0 += w.t1 - w.t0;
+        g0 += t1;
         walk_next<SplitTiling>(p.rag, w);  // there is one: the last unit returned above
+        __syncwarp();
+        if (lane == 0) *ws = w;
+        __syncwarp();
     }
 }
 
