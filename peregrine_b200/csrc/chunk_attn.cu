@@ -1231,8 +1231,11 @@ __device__ __forceinline__ int64_t fragment_at(const FinishParams &p, int i) {
 }
 
 // Behind the pair kernel: block (share, y) joins rows [32 y, +32) of the unit that the share's end cuts.
-// Lane = row and a warp per 16 dims, as the partials lie; the joined rows go out through shared memory.
-__global__ void __launch_bounds__(kFinishThreads) chunk_merge_kernel(const FinishParams p) {
+// Lane = row and a warp per 32 dims, as the partials lie, two fragments' loads in flight; the joined
+// rows go out through shared memory.
+constexpr int kMergeThreads = 256;
+
+__global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const FinishParams p) {
     __shared__ float rows_s[32][kHeadDim + 1];
     pdl_trigger();
     pdl_wait();
@@ -1242,35 +1245,45 @@ __global__ void __launch_bounds__(kFinishThreads) chunk_merge_kernel(const Finis
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int r = blockIdx.y * 32 + lane;
     const int np = f.last - f.first + 1;
-    // fragment i: slot 1 of the first share, then slot 0 of the next ones
-    auto part = [&](int i) { return p.parts + (int64_t)((f.first + i) * 2 + (i == 0 ? 1 : 0)) * kPairPart; };
+    constexpr int kQuads = kHeadDim / 4 / (kMergeThreads / 32);  // of 4 dims, a warp's
     float ma = -INFINITY, den = 0.f;
-    float4 acc[4];
+    float4 acc[kQuads];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-    for (int i = 0; i < np; ++i) {
-        const float *pc = part(i);
-        const float m = pc[kPairStat + r], l = pc[kPairStat + 2 * kBM + r];
-        const float4 *o = reinterpret_cast<const float4 *>(pc) + r;
-        const float4 v[4] = {o[(warp * 4) * 2 * kBM], o[(warp * 4 + 1) * 2 * kBM], o[(warp * 4 + 2) * 2 * kBM], o[(warp * 4 + 3) * 2 * kBM]};
-        if (m == -INFINITY) continue;  // the fragment saw nothing
-        const float mx = fmaxf(ma, m);
-        const float corr = exp2f((ma - mx) * kLog2e), w = exp2f((m - mx) * kLog2e);
+    for (int k = 0; k < kQuads; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < np; i0 += 2) {
+        float m[2], l[2];
+        float4 v[2][kQuads];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            // fragment i: slot 1 of the first share, then slot 0 of the next ones; past the last the
+            // first of the two again, with weight 0
+            const int i = i0 + j < np ? i0 + j : i0;
+            const float *pc = p.parts + (int64_t)((f.first + i) * 2 + (i == 0 ? 1 : 0)) * kPairPart;
+            m[j] = pc[kPairStat + r];
+            l[j] = pc[kPairStat + 2 * kBM + r];
+            if (i0 + j >= np) m[j] = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < kQuads; ++k)
+                v[j][k] = reinterpret_cast<const float4 *>(pc)[(warp * kQuads + k) * 2 * kBM + r];
+        }
+        const float mx = fmaxf(ma, fmaxf(m[0], m[1]));
+        const float base_m = mx == -INFINITY ? 0.f : mx;  // nothing seen so far: all weights 0
+        const float corr = exp2f((ma - base_m) * kLog2e);
+        const float w0 = exp2f((m[0] - base_m) * kLog2e), w1 = exp2f((m[1] - base_m) * kLog2e);
         ma = mx;
-        den = den * corr + l * w;
+        den = den * corr + (l[0] * w0 + l[1] * w1);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            acc[k].x = acc[k].x * corr + v[k].x * w;
-            acc[k].y = acc[k].y * corr + v[k].y * w;
-            acc[k].z = acc[k].z * corr + v[k].z * w;
-            acc[k].w = acc[k].w * corr + v[k].w * w;
+        for (int k = 0; k < kQuads; ++k) {
+            acc[k].x = acc[k].x * corr + (v[0][k].x * w0 + v[1][k].x * w1);
+            acc[k].y = acc[k].y * corr + (v[0][k].y * w0 + v[1][k].y * w1);
+            acc[k].z = acc[k].z * corr + (v[0][k].z * w0 + v[1][k].z * w1);
+            acc[k].w = acc[k].w * corr + (v[0][k].w * w0 + v[1][k].w * w1);
         }
     }
     const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        float *to = &rows_s[lane][warp * 16 + 4 * k];
+    for (int k = 0; k < kQuads; ++k) {
+        float *to = &rows_s[lane][(warp * kQuads + k) * 4];
         to[0] = acc[k].x * inv;
         to[1] = acc[k].y * inv;
         to[2] = acc[k].z * inv;
@@ -1279,10 +1292,10 @@ __global__ void __launch_bounds__(kFinishThreads) chunk_merge_kernel(const Finis
     if (warp == 0 && p.lse != nullptr && r < nrows)
         p.lse[(int64_t)(f.row + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup] = (den == 0.f) ? -INFINITY : ma + logf(den);
     __syncthreads();
-    // warp w: rows 2 w and 2 w + 1; lane l dims [8 l, 8 l + 8)
+    // warp w: rows 4 w to 4 w + 3; lane l dims [8 l, 8 l + 8)
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int rr = 2 * warp + q, row = blockIdx.y * 32 + rr;
+    for (int q = 0; q < 4; ++q) {
+        const int rr = 4 * warp + q, row = blockIdx.y * 32 + rr;
         if (row >= nrows) break;
         const int64_t orow = (int64_t)(f.row + row / kGroup) * kNumQHeads + kvh * kGroup + row % kGroup;
         float v[8];
@@ -1574,7 +1587,7 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
     pp.parts = reinterpret_cast<float *>(ws + lay.parts);
     pp.scale_log2 = scale * kLog2e;
     cudaError_t e = launch_pdl(chunk_pair_kernel, dim3(2 * lay.shares), dim3(kPairThreads), PairSmem::kBytes, stream, tq, tk, tv, pp);
-    if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel, dim3(lay.shares, lay.rows / 32), dim3(kFinishThreads), 0, stream, fp);
+    if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel, dim3(lay.shares, lay.rows / 32), dim3(kMergeThreads), 0, stream, fp);
     if (e != cudaSuccess || weights == nullptr) return e;
     return launch_chunk_weights(q, tk, num_pages, block_tables, max_pages_per_seq, rag, scale, lse, *weights, sm_count, stream);
 }
