@@ -1230,13 +1230,14 @@ __device__ __forceinline__ int64_t fragment_at(const FinishParams &p, int i) {
     return (int64_t)(i == 0 ? 1 : 2 * i) * p.rows * kPartial;
 }
 
-// Behind the pair kernel: block (share, y) joins rows [32 y, +32) of the unit that the share's end cuts.
-// Lane = row and a warp per 32 dims, as the partials lie, two fragments' loads in flight; the joined
-// rows go out through shared memory.
+// Behind the pair kernel: block (share, y, z) joins rows [32 y, +32) and dims [64 z, +64) of the unit that
+// the share's end cuts. Lane = row and a warp per 8 dims, as the partials lie, four fragments' loads in
+// flight; the joined rows go out through shared memory.
 constexpr int kMergeThreads = 256;
+constexpr int kMergeDims = 64;
 
 __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const FinishParams p) {
-    __shared__ float rows_s[32][kHeadDim + 1];
+    __shared__ float rows_s[32][kMergeDims + 1];
     pdl_trigger();
     pdl_wait();
     const Fragment f = read_record(p, blockIdx.x);
@@ -1245,75 +1246,77 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const Finish
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int r = blockIdx.y * 32 + lane;
     const int np = f.last - f.first + 1;
-    constexpr int kQuads = kHeadDim / 4 / (kMergeThreads / 32);  // of 4 dims, a warp's
+    constexpr int kFrags = 4;
+    const int quad = blockIdx.z * (kMergeDims / 4) + warp * 2;  // the warp's two groups of 4 dims
     float ma = -INFINITY, den = 0.f;
-    float4 acc[kQuads];
+    float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    for (int i0 = 0; i0 < np; i0 += kFrags) {
+        float m[kFrags], l[kFrags];
+        float4 v[kFrags][2];
 #pragma unroll
-    for (int k = 0; k < kQuads; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < np; i0 += 2) {
-        float m[2], l[2];
-        float4 v[2][kQuads];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < kFrags; ++j) {
             // fragment i: slot 1 of the first share, then slot 0 of the next ones; past the last the
-            // first of the two again, with weight 0
+            // first of these again, with weight 0
             const int i = i0 + j < np ? i0 + j : i0;
             const float *pc = p.parts + (int64_t)((f.first + i) * 2 + (i == 0 ? 1 : 0)) * kPairPart;
-            m[j] = pc[kPairStat + r];
+            m[j] = i0 + j < np ? pc[kPairStat + r] : -INFINITY;
             l[j] = pc[kPairStat + 2 * kBM + r];
-            if (i0 + j >= np) m[j] = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < kQuads; ++k)
-                v[j][k] = reinterpret_cast<const float4 *>(pc)[(warp * kQuads + k) * 2 * kBM + r];
+            for (int k = 0; k < 2; ++k) v[j][k] = reinterpret_cast<const float4 *>(pc)[(quad + k) * 2 * kBM + r];
         }
-        const float mx = fmaxf(ma, fmaxf(m[0], m[1]));
-        const float base_m = mx == -INFINITY ? 0.f : mx;  // nothing seen so far: all weights 0
-        const float corr = exp2f((ma - base_m) * kLog2e);
-        const float w0 = exp2f((m[0] - base_m) * kLog2e), w1 = exp2f((m[1] - base_m) * kLog2e);
-        ma = mx;
-        den = den * corr + (l[0] * w0 + l[1] * w1);
+        float mx = ma;
 #pragma unroll
-        for (int k = 0; k < kQuads; ++k) {
-            acc[k].x = acc[k].x * corr + (v[0][k].x * w0 + v[1][k].x * w1);
-            acc[k].y = acc[k].y * corr + (v[0][k].y * w0 + v[1][k].y * w1);
-            acc[k].z = acc[k].z * corr + (v[0][k].z * w0 + v[1][k].z * w1);
-            acc[k].w = acc[k].w * corr + (v[0][k].w * w0 + v[1][k].w * w1);
+        for (int j = 0; j < kFrags; ++j) mx = fmaxf(mx, m[j]);
+        const float base_m = mx == -INFINITY ? 0.f : mx;  // nothing seen so far: all weights 0
+        const float corr = fast_exp2((ma - base_m) * kLog2e);
+        ma = mx;
+        den *= corr;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) acc[k] = make_float4(acc[k].x * corr, acc[k].y * corr, acc[k].z * corr, acc[k].w * corr);
+#pragma unroll
+        for (int j = 0; j < kFrags; ++j) {
+            const float w = fast_exp2((m[j] - base_m) * kLog2e);
+            den += l[j] * w;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                acc[k].x += v[j][k].x * w;
+                acc[k].y += v[j][k].y * w;
+                acc[k].z += v[j][k].z * w;
+                acc[k].w += v[j][k].w * w;
+            }
         }
     }
     const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
-    for (int k = 0; k < kQuads; ++k) {
-        float *to = &rows_s[lane][(warp * kQuads + k) * 4];
+    for (int k = 0; k < 2; ++k) {
+        float *to = &rows_s[lane][warp * 8 + 4 * k];
         to[0] = acc[k].x * inv;
         to[1] = acc[k].y * inv;
         to[2] = acc[k].z * inv;
         to[3] = acc[k].w * inv;
     }
-    if (warp == 0 && p.lse != nullptr && r < nrows)
+    if (warp == 0 && blockIdx.z == 0 && p.lse != nullptr && r < nrows)
         p.lse[(int64_t)(f.row + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup] = (den == 0.f) ? -INFINITY : ma + logf(den);
     __syncthreads();
-    // warp w: rows 4 w to 4 w + 3; lane l dims [8 l, 8 l + 8)
+    // 8 threads a row, 8 dims each
+    const int rr = threadIdx.x >> 3, row = blockIdx.y * 32 + rr, d = (threadIdx.x & 7) * 8;
+    if (row >= nrows) return;
+    const int64_t at = ((int64_t)(f.row + row / kGroup) * kNumQHeads + kvh * kGroup + row % kGroup) * kHeadDim + blockIdx.z * kMergeDims + d;
+    float v[8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int rr = 4 * warp + q, row = blockIdx.y * 32 + rr;
-        if (row >= nrows) break;
-        const int64_t orow = (int64_t)(f.row + row / kGroup) * kNumQHeads + kvh * kGroup + row % kGroup;
-        float v[8];
+    for (int k = 0; k < 8; ++k) v[k] = rows_s[rr][d + k];
+    if (p.gate != nullptr) {
+        const uint4 gq = *reinterpret_cast<const uint4 *>(p.gate + at);
+        const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = rows_s[rr][8 * lane + k];
-        if (p.gate != nullptr) {
-            const uint4 gq = *reinterpret_cast<const uint4 *>(p.gate + orow * kHeadDim + 8 * lane);
-            const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w};
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = sigmoid_gate(v[k], (gw[k >> 1] >> ((k & 1) * 16)) & 0xffffu);
-        }
-        uint4 o;
-        o.x = pack_bf16x2(v[0], v[1]);
-        o.y = pack_bf16x2(v[2], v[3]);
-        o.z = pack_bf16x2(v[4], v[5]);
-        o.w = pack_bf16x2(v[6], v[7]);
-        *reinterpret_cast<uint4 *>(p.out + orow * kHeadDim + 8 * lane) = o;
+        for (int k = 0; k < 8; ++k) v[k] = sigmoid_gate(v[k], (gw[k >> 1] >> ((k & 1) * 16)) & 0xffffu);
     }
+    uint4 o;
+    o.x = pack_bf16x2(v[0], v[1]);
+    o.y = pack_bf16x2(v[2], v[3]);
+    o.z = pack_bf16x2(v[4], v[5]);
+    o.w = pack_bf16x2(v[6], v[7]);
+    *reinterpret_cast<uint4 *>(p.out + at) = o;
 }
 
 // One row of a cut unit behind the split kernel, by a block: the fragments (64 and more of a single long
@@ -1587,7 +1590,7 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
     pp.parts = reinterpret_cast<float *>(ws + lay.parts);
     pp.scale_log2 = scale * kLog2e;
     cudaError_t e = launch_pdl(chunk_pair_kernel, dim3(2 * lay.shares), dim3(kPairThreads), PairSmem::kBytes, stream, tq, tk, tv, pp);
-    if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel, dim3(lay.shares, lay.rows / 32), dim3(kMergeThreads), 0, stream, fp);
+    if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel, dim3(lay.shares, lay.rows / 32, kHeadDim / kMergeDims), dim3(kMergeThreads), 0, stream, fp);
     if (e != cudaSuccess || weights == nullptr) return e;
     return launch_chunk_weights(q, tk, num_pages, block_tables, max_pages_per_seq, rag, scale, lse, *weights, sm_count, stream);
 }
