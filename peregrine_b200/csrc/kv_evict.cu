@@ -366,15 +366,18 @@ cudaError_t launch_evict_select(const float *weights, float *weights_out, int64_
     p.keep_last = keep_last;
     p.kept = kept;
     p.new_lens = new_lens;
-    // Threads and CTAs per row: at least what keeps a thread within kMaxPer weights, 512 threads while
-    // they suffice (two CTAs an SM overlap their barriers and loads); a batch that leaves SMs free
-    // takes more CTAs, up to 8, down to kSplitPer weights a thread, below which the cluster's barriers
-    // cost more than they save.
-    constexpr int kSplitPer = 8;
+    // Threads and CTAs per row: at least what keeps a thread within kMaxPer weights, 1024 threads from
+    // kLongRow tokens on (fewer barriers across the cluster: 60.9 us against 63.5 for 64 rows of up to
+    // 65536), else 512 (two CTAs an SM: 32.2 us against 50.0 for 800 rows of up to 8192); a batch that
+    // leaves SMs free takes more CTAs, up to 8, down to kSplitPer weights a thread, below which the
+    // cluster's barriers cost more than they save. A CTA a row that reads it from L2 for every round
+    // instead took 146 and 51 us.
+    constexpr int kSplitPer = 8, kLongRow = 32768;
+    static_assert(kLongRow <= 8 * 512 * kMaxPer, "512 threads must hold the shorter rows");
     int sms = 148, dev = 0;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const int threads = max_seq_len > 8 * 512 * kMaxPer ? 1024 : 512;
+    const int threads = max_seq_len > kLongRow ? 1024 : 512;
     auto weights_per_thread = [&](int c) { return (int)(((int64_t)max_seq_len + (int64_t)c * threads - 1) / ((int64_t)c * threads)); };
     int ctas = 1;
     while (ctas < 8 && (weights_per_thread(ctas) > kMaxPer ||
