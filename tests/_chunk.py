@@ -80,7 +80,8 @@ def reference(c):
       (a thread sums at most L / 32 terms one after the other, the rest pairwise);
       lse: ds + (L / 32 + 40) e + e |lse|;
       out: the rounded P gives u sum p|v|, the statistics dp sum p|v|, the output rounding u |o| and
-      the gate's sigmoid 4 ulp;
+      the gate's sigmoid (4 + 2 |gate|) ulp: an approximate exponential (2), reciprocal (1) and a product,
+      the exponent's rounding |gate| log2(e) half ulps;
       weights: dp + (rows of the sum) e, relative."""
     u, e = 2.0 ** -8, 2.0 ** -23
     dev = dict(dtype=torch.float64, device="cuda")
@@ -106,11 +107,12 @@ def reference(c):
                     p = (s - t).exp().masked_fill(hidden, 0)  # nothing visible: 0
                     dp = 2 * ds + (L / 32 + 40) * e
                     o, av = p @ v, p @ v.abs()
-                    sig = 1.0
+                    sig, gulp = 1.0, 4.0
                     if c["gate"] is not None:
                         sig = torch.sigmoid(c["gate"][r0 + a:r0 + z, g].double())
+                        gulp = 4 + 2 * c["gate"][r0 + a:r0 + z, g].double().abs()
                     out[r0 + a:r0 + z, g] = o * sig
-                    tol[r0 + a:r0 + z, g] = (u + dp) * av * sig + (u + 4 * e) * (o * sig).abs() + 1e-30
+                    tol[r0 + a:r0 + z, g] = (u + dp) * av * sig + (u + gulp * e) * (o * sig).abs() + 1e-30
                     lse[r0 + a:r0 + z, g] = t[:, 0]
                     ltol[r0 + a:r0 + z, g] = (ds + (L / 32 + 40) * e + e * torch.where(t.isinf(), 0, t.abs()))[:, 0]
                     w[h] += p.sum(0)
