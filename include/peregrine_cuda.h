@@ -267,6 +267,7 @@ size_t pgc_chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_
  *   gate       nullable [total_q][16][256] bf16: out = attn * sigmoid(gate)
  *   out        [total_q][16][256] bf16
  *   lse        nullable [total_q][16] fp32: log of the row's sum of exp(scale q.k), before the gate
+ *   scale      > 0
  * Row i of a sequence of n rows sits at position seq_lens[b] - n + i and sees the tokens up to it; a
  * row at a negative position (seq_lens[b] < n) sees nothing: out 0, lse -inf. Rows before q_starts[0]
  * and from q_starts[batch] on are left as they were. total_q, max_q_len and max_seq_len are
@@ -276,8 +277,10 @@ size_t pgc_chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_
  * A masked token's score is never used, whatever it is, and slots past a sequence's end are never
  * read into a sum; but a NaN or infinite V element of a cached token of the sequence makes that output
  * dim NaN in rows before the token too (its probability there is 0, and 0 times it is NaN).
- * q, k/v_pages, gate, out and workspace 16-byte aligned. Calls that may overlap on the GPU, and
- * graphs that may, need workspaces of their own. */
+ * q, k/v_pages, gate, out and workspace 16-byte aligned; out, lse and the workspace overlap no input.
+ * Calls that may overlap on the GPU, and graphs that may, need workspaces of their own. The work is
+ * dealt out by the whole batch's lengths: the same batch gives the same bits every time, a sequence
+ * in another batch the same values within rounding. */
 int pgc_chunk_attn(const uint16_t *q, const uint16_t *k_pages, const uint16_t *v_pages,
                    int64_t num_pages, const int32_t *block_tables, int max_pages_per_seq,
                    const int32_t *q_starts, const int32_t *seq_lens, int batch, int total_q,

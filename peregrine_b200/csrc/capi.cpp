@@ -500,7 +500,7 @@ static int chunk_call(const uint16_t *q, const uint16_t *k_pages, const uint16_t
                       void *workspace, size_t workspace_bytes, void *stream) {
     // arguments are checked before the device is asked for, so refusals need no GPU
     if (batch < 0 || total_q < 0 || max_q_len < 0 || max_seq_len < 0 || num_pages <= 0 || max_pages_per_seq < 0 ||
-        !std::isfinite(scale))
+        !std::isfinite(scale) || !(scale > 0.f))
         return PGC_ERR_INVALID;
     if (batch > PGC_CHUNK_MAX_BATCH) return PGC_ERR_BOUNDS;
     if (weights && (weights->stride < max_seq_len || weights->num_slots <= 0 ||

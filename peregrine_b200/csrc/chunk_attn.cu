@@ -8,14 +8,18 @@
 // exp(s_t - lse). A row that sees nothing (p < 0) has o = 0 and lse = -inf.
 //
 // Two forms, chosen by the host bound on the rows of a sequence:
-//   * up to PGC_MAX_QUERIES rows: chunk_split_kernel (mma.sync), bound by the K/V bytes; with weights
-//     it leaves the scores in the workspace and chunk_add_kernel turns them into weights, so K is
-//     read once;
-//   * more rows: chunk_pair_kernel on the 5th-gen tensor cores, and chunk_weights.cu for the weights.
+//   * up to PGC_MAX_QUERIES rows: chunk_split_kernel (mma.sync), bound by the K/V bytes (64 sequences of
+//     1024 to 32768 tokens, 2.1 GB: 323 us, 6.5 TB/s); with weights it leaves the scores in the
+//     workspace, 16 B per row, kv head and token beside 1 KiB of K and V, so that K is read once;
+//   * more rows: chunk_pair_kernel on the 5th-gen tensor cores (1600 tokens over 24576: 496 us, 1340
+//     TFLOP/s), and chunk_weights.cu for the weights.
 // In both, the line of all the batch's tiles is cut into equal consecutive shares, one per CTA (or
-// pair) of a fixed grid: lengths are on the device, and the balance is within one tile whatever they
-// are. A unit of work cut by a share's border leaves fp32 partials, at most two units a share (its
-// first and its last), which the merge kernel joins; every other unit is written where it is computed.
+// pair) of a fixed grid: lengths are on the device, and a grid by the host's bounds would be empty for
+// the most part where they are ragged (387 us for the 64 sequences above). A unit of work cut by a
+// share's border leaves fp32 partials, at most two units a share (its first and its last), which a
+// second kernel joins; every other unit is written where it is computed.
+// One-row calls of one or a few sequences are bound by latency, about 16 us for 4097 tokens: 2 us to
+// the first load, 4 to 6 of loads, 2 for the join in the CTA, 5 for the second kernel.
 #include <cuda.h>
 
 #include "pgc_common.cuh"
@@ -320,7 +324,8 @@ struct SplitSmem {
     static constexpr int kBar = kL + kConsumers * kRows * 4;  // full[4], empty[4], q_full[2], q_empty[2]
     static constexpr int kWalk = kBar + (2 * kStages + 4) * 8;  // per consumer warp
     static constexpr int kLine = kWalk + kConsumers * sizeof(Walk);
-    static constexpr int kBytes = kLine + 24;
+    static constexpr int kAbort = kLine + 24;
+    static constexpr int kBytes = kAbort + 8;
 };
 constexpr int kSplitSmem = SplitSmem::kBytes + 1024;  // + alignment slack
 static_assert(sizeof(Walk) <= 48 && sizeof(Line) <= 24 && SplitSmem::kWalk % 8 == 0, "schedule slots");
@@ -333,6 +338,12 @@ __device__ __forceinline__ void bulk_load(void *smem_dst, const void *src, uint3
                  ::"r"(smem_u32(smem_dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
 }
+
+// Hands a stage back to the producer once `data`, the last register loaded from it, has arrived: the
+// barrier's address depends on it through a value that is 0 at run time (the grid is one-dimensional).
+// Program order alone did not hold the last ldmatrix before the arrival: about once in 60 000 launches
+// it read the stage's next page in the last 16 dims.
+__device__ __forceinline__ void release_stage(uint64_t *bar, uint32_t data) { mbar_arrive(bar + (data & blockIdx.z)); }
 
 // One (page, kv head) of a pool, by its pool_page_map.
 __device__ __forceinline__ void tma_load_page(void *smem_dst, const void *tmap, int32_t row, uint64_t *bar, uint64_t policy) {
@@ -357,9 +368,14 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     const int lane = threadIdx.x & 31;
     const int index = blockIdx.x;
     Line *line = reinterpret_cast<Line *>(smem + SplitSmem::kLine);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + SplitSmem::kAbort);
+    auto wait = [&](uint64_t *bar, uint32_t parity, int where) {
+        return wait_or_abort(bar, parity, abort_flag, &g_chunk_err, where);
+    };
 
     pdl_trigger();
     if (threadIdx.x == 0) {
+        *abort_flag = 0;
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
@@ -375,8 +391,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     pdl_wait();
     Walk w;
     const bool busy = find_share<SplitTiling>(p.rag, reinterpret_cast<int64_t *>(smem + SplitSmem::kRing), index,
-                                              gridDim.x, reinterpret_cast<Walk *>(smem + SplitSmem::kWalk),
-                                              line,
+                                              gridDim.x, reinterpret_cast<Walk *>(smem + SplitSmem::kWalk), line,
                                               index == 0 ? &g_chunk_err : nullptr, w);
     if (!busy) return;
     fence_proxy_async_smem();  // the schedule's scratch becomes the ring
@@ -390,17 +405,16 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
             const int qb = unit & 1;
             bool ok = true;
             if (lane == 0) {
-                ok = unit < 2 || mbar_wait_bounded(&q_empty[qb], ((unit >> 1) - 1) & 1);
+                ok = unit < 2 || wait(&q_empty[qb], ((unit >> 1) - 1) & 1, 21);
                 if (ok) {
                     mbar_arrive_expect_tx(&q_full[qb], (uint32_t)w.n * kGroup * kHeadDim * 2);
                     for (int r = 0; r < w.n * kGroup; ++r)
                         bulk_load(smem + SplitSmem::kQ + (qb * kRows + r) * kQRowBytes,
                                   p.q + ((int64_t)(w.row0 + r / kGroup) * kNumQHeads + w.kvh * kGroup + r % kGroup) * kHeadDim,
                                   kHeadDim * 2, &q_full[qb]);
-                } else {
-                    record_error(&g_chunk_err, kErrWaitTimeout, 21);
                 }
             }
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0);
             const int32_t *table = p.block_tables + (int64_t)w.seq * p.max_pages_per_seq;
             int ids = 0;
             for (int t = w.t0; ok && t < w.t1; ++t, ++g) {
@@ -418,8 +432,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
                 const int page = __shfl_sync(0xffffffffu, ids, k);
                 if (lane == 0) {
                     const int s = g % kStages, round = g / kStages;
-                    if (round > 0 && !mbar_wait_bounded(&empty[s], (round - 1) & 1)) {
-                        record_error(&g_chunk_err, kErrWaitTimeout, 22);
+                    if (round > 0 && !wait(&empty[s], (round - 1) & 1, 22)) {
                         ok = false;
                     } else if (t * kPage < w.len) {
                         uint8_t *stage = smem + SplitSmem::kRing + s * kStageBytes;
@@ -433,7 +446,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
                 }
                 ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0);
             }
-            if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) || !walk_next<SplitTiling>(p.rag, w)) break;
+            if (!ok || !walk_next<SplitTiling>(p.rag, w)) break;
         }
         return;
     }
@@ -468,16 +481,13 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-        // A wait that gives up is recorded and the warp runs on (every later wait is bounded too), so
+        // A wait that gives up is recorded and the warp runs on, every later wait returning at once, so
         // that the four warps stay in step at their barriers.
-        if (!mbar_wait_bounded(&q_full[qb], (unit >> 1) & 1)) record_error(&g_chunk_err, kErrWaitTimeout, 23);
+        wait(&q_full[qb], (unit >> 1) & 1, 23);
         for (int t = ws->t0 + ((warp - g0 - ws->t0) & (kConsumers - 1)); t < t1; t += kConsumers) {
             const int g = g0 + t;  // g % 4 == warp
             const int s = g % kStages;
-            if (!mbar_wait_bounded(&full[s], (g / kStages) & 1)) {
-                record_error(&g_chunk_err, kErrWaitTimeout, 24);
-                break;
-            }
+            if (!wait(&full[s], (g / kStages) & 1, 24)) break;
             uint8_t *kt = smem + SplitSmem::kRing + s * kStageBytes;
             uint8_t *vt = kt + kTileBytes;
             const uint32_t k_base = smem_u32(kt);
@@ -576,15 +586,15 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
             }
 
             // O[16 x 256] += P[16 x 16] V[16 x 256]
+            uint32_t b0, b1, b2, b3;
 #pragma unroll
             for (int nd = 0; nd < 16; ++nd) {
-                uint32_t b0, b1, b2, b3;
                 ldsm_x4_trans(v_base + swz_page_offset(v_tok, nd * 16 + v_dim_off), b0, b1, b2, b3);
                 mma_bf16_16816(o[2 * nd], pa0, pa1, pa2, pa3, b0, b1);
                 mma_bf16_16816(o[2 * nd + 1], pa0, pa1, pa2, pa3, b2, b3);
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[s]);
+            if (lane == 0) release_stage(&empty[s], b3);
         }
 
         // ------------------------------------------------------------ join the 4 warp states
@@ -807,8 +817,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     Walk w;
     const bool busy = find_share<PairTiling>(p.rag, reinterpret_cast<int64_t *>(smem + PairSmem::kK), pair, gridDim.x >> 1,
                                              reinterpret_cast<Walk *>(smem + PairSmem::kWalk),
-                                             line,
-                                             blockIdx.x == 0 ? &g_chunk_err : nullptr, w);
+                                             line, blockIdx.x == 0 ? &g_chunk_err : nullptr, w);
     // the record of the share, that no unit is cut by its end until its walk has ended
     if (leader && threadIdx.x == 0) p.frags[pair].last = p.frags[pair].first = 0;
     if (!busy) return;  // both CTAs of the pair

@@ -17,6 +17,9 @@ SMALL = {
     "only_nothing": [(1, 0), (0, 0)],
     "long": [(1, 20000), (1, 100), (2, 7)],
     "many": [(1 + i % 4, 5 + 37 * i) for i in range(40)],
+    "no_rows": [(0, 5), (0, 0)],
+    "batch_129": [(i % 5, 3 + 5 * (i % 97)) for i in range(129)],
+    "batch_4096": [(1 + i % 2, 1 + i % 40) if i % 8 == 0 else (0, 3) for i in range(4096)],
 }
 LARGE = {
     "five": [(5, 5)],
@@ -28,6 +31,8 @@ LARGE = {
     "tiny_chunks": [(5 + i % 60, 200 + 31 * i) for i in range(40)],
     "chunk_from_nothing": [(1000, 1000)],
     "decode_among_chunks": [(1, 700), (300, 900), (1, 1), (4, 5000), (0, 0), (129, 130)],
+    "batch_300": [(i % 9, 9 + 7 * (i % 61)) for i in range(300)],
+    "batch_4096_chunks": [(5, 5 + i % 30) if i % 8 == 0 else (0, 7) for i in range(4096)],
 }
 
 
@@ -44,6 +49,27 @@ def test_against_reference(cuda, name, weights):
     got = call(cuda, c, weights=w)
     torch.cuda.synchronize()
     assert cuda.device_error() == (0, 0)
+    check(c, got, reference(c), w, before)
+
+
+def test_no_rows_in_chunk_form(cuda):
+    """Rows of nobody only: nothing is written."""
+    import torch
+    c = make([(0, 40), (0, 0)], seed=3, first_row=2, rows_behind=6)
+    w = torch.ones((2, NKV, 40), device="cuda")
+    out, lse = call(cuda, c, weights=w, qmax=64)
+    torch.cuda.synchronize()
+    assert (out.float() == 7.0).all() and (lse == -7.0).all() and (w == 1).all()
+    assert cuda.device_error() == (0, 0)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 9])
+def test_very_long_cache(cuda, rows):
+    import torch
+    c = make([(rows, 150001)], seed=rows, gate=True)
+    before = torch.zeros((1, NKV, c["lmax"]), device="cuda")
+    w = before.clone()
+    got = call(cuda, c, weights=w)
     check(c, got, reference(c), w, before)
 
 
@@ -70,6 +96,19 @@ def test_same_bits_every_time(cuda, seqs):
     runs.append((*call(cuda, c), runs[0][2]))
     for r in runs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(runs[0], r))
+
+
+def test_same_bits_over_many_launches(cuda):
+    """A ring stage handed back before its last read is in shows as another bit pattern now and then."""
+    import torch
+    c = make(SMALL["many"], seed=1)
+    want, lse = call(cuda, c)
+    ws = torch.empty(cuda.chunk_workspace_bytes(len(c["seqs"]), c["rows"], c["qmax"], c["lmax"]), dtype=torch.uint8, device="cuda")
+    outs = [want.clone() for _ in range(50)]
+    for _ in range(300):
+        for o in outs:
+            call(cuda, c, out=o, lse=lse, workspace=ws)
+        assert all(torch.equal(o, want) for o in outs)
 
 
 def test_agrees_with_uniform_decode(cuda):

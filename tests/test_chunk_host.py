@@ -34,7 +34,7 @@ def chunk(lib, with_weights, **change):
     (dict(starts=None), INVALID), (dict(lens=None), INVALID), (dict(out=None), INVALID), (dict(ws=None), WORKSPACE),
     (dict(pages=0), INVALID), (dict(batch=-1), INVALID), (dict(rows=-1), INVALID), (dict(qmax=-1), INVALID),
     (dict(lmax=-1), INVALID), (dict(lmax=0), INVALID), (dict(width=-1), INVALID), (dict(width=0), INVALID),
-    (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID), (dict(batch=4097, num_slots=5000), BOUNDS),
+    (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID), (dict(scale=0.0), INVALID), (dict(scale=-0.0625), INVALID), (dict(batch=4097, num_slots=5000), BOUNDS),
     (dict(width=9), BOUNDS), (dict(pages=1 << 25), BOUNDS), (dict(rows=(1 << 22) + 1), BOUNDS),
     (dict(lmax=(1 << 24) + 1, width=1 << 21, stride=1 << 25), BOUNDS), (dict(ws_bytes=0), WORKSPACE),
     (dict(q=A + 8), ALIGN), (dict(k=A + 2), ALIGN), (dict(v=A + 4), ALIGN), (dict(gate=A + 8), ALIGN),
@@ -67,8 +67,8 @@ def test_workspace_grows_with_the_shape(lib):
     assert f(2, 8, 4, 160, 1) > f(2, 8, 4, 160, 0)
     scores, lse = 8 * 4 * (1 << 15) * 4 * 4, 8 * 16 * 4
     assert f(2, 8, 4, 1 << 15, 1) - f(2, 8, 4, 1 << 15, 0) == scores + lse
-    assert f(2, 8, 4, 1 << 20, 0) == f(4096, 1 << 12, 4, 100, 0) <= 10 << 20
-    assert f(4096, 1 << 20, 512, 1 << 20, 0) == f(1, 5, 5, 100, 0) <= 38 << 20
+    assert f(2, 8, 4, 1 << 20, 0) == f(2, 1 << 12, 4, 100, 0) <= 10 << 20
+    assert f(4096, 1 << 20, 512, 1 << 20, 0) == f(1, 5, 5, 100, 0) <= 39 << 20
 
 
 SELECT = dict(w=A, wo=None, stride=160, num_slots=2, slots=None, lens=A, batch=2, lmax=160, budget=32, first=4, last=8,
