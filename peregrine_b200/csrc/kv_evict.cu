@@ -18,19 +18,20 @@ PGC_DEFINE_ERROR_WORD(g_evict_err);
 namespace {
 
 // ---------------------------------------------------------------- selection
-// A cluster of 1-8 CTAs per (sequence, kv head). Each warp holds a segment of the row in registers, as
-// order-preserving integers: the first and last tokens as the greatest, places past the row's end as
-// the smallest, so that one rule serves all. The value of rank B is found from its top byte down: a
-// histogram of the next byte of the values that share the bytes found so far, summed over the cluster
-// through distributed shared memory, up to four times; it stops when all that share them are kept.
-// Then the warps count what they keep, the counts are scanned over warps and CTAs, and the tokens are
-// written in order.
-// The histogram has a column per lane: lane l adds to hist[byte][l], its own bank, so a warp's adds
+// A cluster of 1-8 CTAs per (sequence, kv head); a row that fewer can hold uses fewer. Each warp holds a
+// segment of the row in registers, as order-preserving integers, all but the first F and the last R
+// tokens, which are kept anyway. The least value kept among the others is searched for in a range that
+// shrinks: a histogram over 256 equal parts of it, summed over the cluster through distributed shared
+// memory, says which part holds the value. The first range is the non-negative floats (a part is an
+// octave). When few values are left in the range, they are listed and ranked against one another; when
+// all that are left are kept, the search is over. Then the warps count what they keep, the counts are
+// scanned over warps and CTAs, and the tokens are written in order.
+// The histogram has a column per lane: lane l adds to hist[part][l], its own bank, so a warp's adds
 // never meet however the weights cluster (attention weights share a few exponents; with one shared
-// column those adds ran one after the other: 519 us for 64 sequences of up to 65536 tokens). What
-// bounds the kernel is the instructions issued, some 50 per 32 weights, and the cluster barriers.
+// column those adds ran one after the other: 519 us for 64 sequences of up to 65536 tokens).
 constexpr int kBins = 256;
 constexpr int kMaxPer = 32;  // weights a thread
+constexpr int kListed = 256;  // values that are ranked against one another
 static_assert(8 * 1024 * kMaxPer >= PGC_EVICT_MAX_TOKENS, "the longest row does not fit a cluster");
 
 struct SelectParams {
@@ -41,13 +42,14 @@ struct SelectParams {
     const int32_t *seq_lens;
     int max_seq_len;
     int budget, keep_first, keep_last;
+    int share;  // weights a CTA takes before another one of its cluster joins in
     int32_t *kept;
     int32_t *new_lens;
 };
 
-// A weight as it is held and moved: -0 as +0, every NaN as the one whose order bits are 0.
-__device__ __forceinline__ float canonical(float x) { return x == x ? x + 0.f : __uint_as_float(0xffffffffu); }
-// Unsigned integers in the order of the canonical floats, NaN below everything.
+// A weight as it is held and moved: -0 as +0, every NaN as the one whose order bits are 1.
+__device__ __forceinline__ float canonical(float x) { return x == x ? x + 0.f : __uint_as_float(0xfffffffeu); }
+// Unsigned integers in the order of the canonical floats, NaN below everything, 0 for none.
 __device__ __forceinline__ uint32_t order_bits(float x) {
     const int32_t u = __float_as_int(x);
     return (uint32_t)u ^ ((uint32_t)(u >> 31) | 0x80000000u);
@@ -76,26 +78,22 @@ __device__ __forceinline__ uint32_t load_peer(const void *p, uint32_t cta) {
 
 template <int kSelThreads, int kPer>  // kPer: weights a thread, at most
 __global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_kernel(const SelectParams p) {
-    constexpr int kSelWarps = kSelThreads / 32;
-    extern __shared__ uint32_t dyn[];
+    constexpr int kSelWarps = kSelThreads / 32, kPartThreads = kSelThreads / kBins;
+    extern __shared__ __align__(16) uint32_t dyn[];
     uint32_t *hist = dyn;                                       // [256][32 lanes]
     float *vals = reinterpret_cast<float *>(dyn + kBins * 32);  // this CTA's share of the weights
     __shared__ uint32_t totals[2][kBins];  // this CTA's histogram, read by the cluster
-    __shared__ uint32_t warp_sum[kBins / 32];
-    __shared__ uint32_t found[3];  // the byte, the values above it and of it
+    __shared__ uint32_t warp_sum[kSelWarps];
+    __shared__ uint32_t found[3];  // the part, the values above it and of it
     __shared__ uint32_t cnt[2];    // values above the ties in this CTA, and ties
     __shared__ uint32_t seg_sure[kSelWarps], seg_tie[kSelWarps];
+    __shared__ uint32_t listed, list[kListed];  // this CTA's values of the last range, read by the cluster
+    __shared__ uint32_t all[kListed];           // the cluster's
     pdl_trigger();
     pdl_wait();
-    const uint32_t rank = cta_in_cluster(), ctas = ctas_in_cluster();
+    const uint32_t rank = cta_in_cluster(), cluster = ctas_in_cluster();
     const int h = blockIdx.y, b = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    auto sync_all = [&]() {
-        if (ctas > 1)
-            cluster_sync();
-        else
-            __syncthreads();
-    };
     const bool reporter = h == 0 && rank == 0;
     int32_t *kept = p.kept + ((int64_t)b * kNumKvHeads + h) * p.budget;
 
@@ -109,24 +107,34 @@ __global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_
     const int B = p.budget;
     const int n_new = min(L, B);
     if (reporter && tid == 0 && p.new_lens != nullptr) p.new_lens[b] = n_new;
-    for (int i = n_new + (int)rank * kSelThreads + tid; i < B; i += (int)ctas * kSelThreads) kept[i] = -1;
+    for (int i = n_new + (int)rank * kSelThreads + tid; i < B; i += (int)cluster * kSelThreads) kept[i] = -1;
     const int64_t row = (max(slot, (int64_t)0) * kNumKvHeads + h) * p.stride;
     const float *w = p.weights + row;
     float *wo = p.weights_out != nullptr ? p.weights_out + row : nullptr;
     if (L <= B) {  // uniform over the cluster
-        for (int i = (int)rank * kSelThreads + tid; i < L; i += (int)ctas * kSelThreads) {
+        for (int i = (int)rank * kSelThreads + tid; i < L; i += (int)cluster * kSelThreads) {
             kept[i] = i;
             if (wo != nullptr && wo != w) wo[i] = w[i];
         }
         return;
     }
 
+    // the CTAs that this row uses; the cluster's barriers do not wait for those that have left
+    const uint32_t ctas = (uint32_t)min((int)cluster, (L + p.share - 1) / p.share);
+    if (rank >= ctas) return;
+    auto sync_all = [&]() {
+        if (ctas > 1)
+            cluster_sync();
+        else
+            __syncthreads();
+    };
+
     // warp segments of `per` x 32 consecutive weights; element j of a lane is number j * 32 + lane.
     // `per` is a multiple of 4, so that the loops below test it once per 4 elements.
     const int per = (int)(((int64_t)L + (int64_t)ctas * kSelThreads * 4 - 1) / ((int64_t)ctas * kSelThreads * 4)) * 4;
     const int i0 = warp * per * 32 + lane;        // in the CTA's share
     const int t0 = (int)rank * per * kSelThreads;  // the share's first token
-    const int last = L - p.keep_last;
+    const int F = p.keep_first, last = L - p.keep_last;
     uint32_t key[kPer];
 #define PGC_EACH_KEY \
     _Pragma("unroll") for (int j4 = 0; j4 < kPer; j4 += 4) if (j4 < per) _Pragma("unroll") for (int j = j4; j < j4 + 4; ++j)
@@ -136,89 +144,150 @@ __global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_
     }
 #pragma unroll
     for (int i = 0; i < kBins * 32 / kSelThreads; ++i) hist[i * kSelThreads + tid] = 0;
+    if (tid == 0) listed = 0;
     PGC_EACH_KEY {
         const int t = t0 + i0 + j * 32;
         const float x = canonical(__uint_as_float(key[j]));
         if (wo != nullptr) vals[i0 + j * 32] = x;
-        key[j] = t >= L ? 0u : (t < p.keep_first || t >= last) ? 0xffffffffu : order_bits(x);
+        key[j] = (uint32_t)(t - F) < (uint32_t)(last - F) ? order_bits(x) : 0u;
     }
     __syncthreads();
 
-    // Values that begin with the bytes found lie in [tie_lo, tie_lo + tie_width]: the ties; those
-    // above are kept, and `need` of the ties, the first in order. Places past the row's end may tie
-    // with NaN weights only, which come before them.
+    // The value sought is in [lo, lo + width]: what lies above is kept, and `need` of the `ties` inside,
+    // the first in order. With need = 0 the search ends at once, with everything above.
     const uint32_t hist_lane = smem_u32(hist) + lane * 4;
-    uint32_t need = (uint32_t)B, tie_lo = 0, tie_width = 0xffffffffu, ties = 0;
+    uint32_t need = (uint32_t)(B - F - p.keep_last), lo = 0x80000000u, width = 0x7fffffffu, ties = ~0u;
+    if (need == 0) {
+        lo = ~0u;  // no key is as great
+        width = 0;
+        ties = 0;
+    }
 #pragma unroll 1
-    for (int sh = 24; sh >= 0; sh -= 8) {
-        const uint32_t buf = (sh >> 3) & 1;
+    for (uint32_t buf = 0; ties != need && width != 0; buf ^= 1) {
+        if (ties <= (uint32_t)kListed) {
+            PGC_EACH_KEY {
+                if (key[j] - lo <= width) list[atomicAdd(&listed, 1u)] = key[j] - lo;
+            }
+            sync_all();
+            uint32_t v = 0;
+            if (tid < (int)ties) {
+                uint32_t q = 0, at = (uint32_t)tid, n = load_peer(&listed, 0);
+                while (at >= n) {  // the CTAs' lists have `ties` values between them
+                    at -= n;
+                    n = load_peer(&listed, ++q);
+                }
+                v = load_peer(&list[at], q);
+                all[tid] = v;
+            }
+            __syncthreads();
+            if (tid < (int)ties) {
+                uint32_t above = 0, same = 0;
+                for (uint32_t i = 0; i < ties; ++i) {
+                    const uint32_t x = all[i];
+                    above += x > v;
+                    same += x == v;
+                }
+                if (above < need && above + same >= need) {
+                    found[0] = v;
+                    found[1] = above;
+                    found[2] = same;
+                }
+            }
+            __syncthreads();
+            need -= found[1];
+            ties = found[2];
+            lo += found[0];
+            width = 0;
+            break;
+        }
+        const int sh = max(0, 24 - __clz((int)width));
         // predicated adds: a branch around each costs more than the add
         PGC_EACH_KEY {
             asm volatile(
                 "{\n\t.reg .pred in;\n\t"
                 "setp.le.u32 in, %0, %1;\n\t"
                 "@in red.shared.add.u32 [%2], 1;\n\t}"
-                ::"r"(key[j] - tie_lo), "r"(tie_width), "r"(hist_lane + ((key[j] >> sh) & 255u) * 128)
+                ::"r"(key[j] - lo), "r"(width), "r"(hist_lane + ((key[j] - lo) >> sh) * 128)
                 : "memory");
         }
         __syncthreads();
-        // warp w sums the columns of 8 bytes and clears them for the next round
+        // kPartThreads threads sum a part's columns and clear them for the next round, 16 bytes at a
+        // time, each part from another bank group on; the parts go down as the threads go up
+        const int part = kBins - 1 - tid / kPartThreads, sub = tid % kPartThreads;
+        uint32_t c = 0;
 #pragma unroll
-        for (int k = 0; k < kBins / kSelWarps; ++k) {
-            const int bin = warp * (kBins / kSelWarps) + k;
-            const uint32_t sum = __reduce_add_sync(0xffffffffu, hist[bin * 32 + lane]);
-            hist[bin * 32 + lane] = 0;
-            if (lane == 0) totals[buf][bin] = sum;
+        for (int k = 0; k < 8 / kPartThreads; ++k) {
+            uint4 *q = reinterpret_cast<uint4 *>(hist + part * 32) + ((sub * (8 / kPartThreads) + k + part) & 7);
+            const uint4 x = *q;
+            *q = make_uint4(0, 0, 0, 0);
+            c += (x.x + x.y) + (x.z + x.w);
         }
-        // also orders the clearing before the next round's adds; totals are double-buffered, so a
-        // peer's reads of a round are over when this CTA writes that buffer again
-        sync_all();
-        // thread i < 256: byte 255 - i over the cluster, then the sum of those above it
-        uint32_t c = 0, incl = 0;
-        const int bin = kBins - 1 - tid;
-        if (tid < kBins) {
-            if (ctas > 1) {
-                uint32_t v[8];
+        auto part_sum = [](uint32_t x) {
 #pragma unroll
-                for (uint32_t q = 0; q < 8; ++q) v[q] = q < ctas ? load_peer(&totals[buf][bin], q) : 0;
+            for (int o = 1; o < kPartThreads; o *= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
+            return x;
+        };
+        c = part_sum(c);
+        if (ctas > 1) {
+            // totals are double-buffered: a peer's reads of a round are over when this CTA writes that
+            // buffer again
+            if (sub == 0) totals[buf][part] = c;
+            cluster_sync();
+            c = 0;
 #pragma unroll
-                for (uint32_t q = 0; q < 8; ++q) c += v[q];
-            } else {
-                c = totals[buf][bin];
+            for (uint32_t k = 0; k < 8 / kPartThreads; ++k) {
+                const uint32_t q = sub + k * kPartThreads;
+                if (q < ctas) c += load_peer(&totals[buf][part], q);
             }
-            incl = c;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += x;
-            }
-            if (lane == 31) warp_sum[warp] = incl;
+            c = part_sum(c);
         }
+        // the sum of a part and those above it
+        uint32_t incl = sub == 0 ? c : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+        }
+        if (lane == 31) warp_sum[warp] = incl;
         __syncthreads();
-        if (tid < kBins) {
-            uint32_t above = incl - c;
-            for (int q = 0; q < warp; ++q) above += warp_sum[q];
-            if (above < need && above + c >= need) {
-                found[0] = (uint32_t)bin;
-                found[1] = above;
+        incl += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
+        if (sub == 0) {
+            if (incl - c < need && incl >= need) {
+                found[0] = (uint32_t)part;
+                found[1] = incl - c;
                 found[2] = c;
+            }
+            // the first range only: too few there, the value is below it
+            if (part == 0 && incl < need) {
+                found[1] = incl;
+                found[2] = 0;
             }
         }
         __syncthreads();
         need -= found[1];
-        ties = found[2];
-        tie_lo |= found[0] << sh;
-        tie_width = (1u << sh) - 1;
-        if (ties == need) break;  // uniform over the cluster
+        if (found[2] == 0) {  // the negative floats and NaN
+            lo = 1;
+            width = 0x7ffffffeu;
+            ties = ~0u;
+        } else {
+            ties = found[2];
+            lo += found[0] << sh;
+            width = min(width - (found[0] << sh), (1u << sh) - 1);
+        }
     }
 
+    const bool all_ties = ties == need;  // everything from lo on is kept
     uint32_t n_sure = 0, n_tie = 0;
-    PGC_EACH_KEY {
-        n_tie += key[j] - tie_lo <= tie_width;
-        n_sure += key[j] > tie_lo + tie_width;
+    if (all_ties) {
+        PGC_EACH_KEY n_sure += key[j] >= lo;
+    } else {
+        PGC_EACH_KEY {
+            n_tie += key[j] - lo <= width;
+            n_sure += key[j] > lo + width;
+        }
+        n_tie = __reduce_add_sync(0xffffffffu, n_tie);
     }
     n_sure = __reduce_add_sync(0xffffffffu, n_sure);
-    n_tie = __reduce_add_sync(0xffffffffu, n_tie);
     if (lane == 0) {
         seg_sure[warp] = n_sure;
         seg_tie[warp] = n_tie;
@@ -243,12 +312,11 @@ __global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_
         tie_before += __reduce_add_sync(0xffffffffu, e);
     }
     const uint32_t lt = (1u << lane) - 1;
-    const bool all_ties = ties == need;
+    sure_before += (uint32_t)F;
     if (all_ties) {
-        // everything from tie_lo on is kept
-        uint32_t at = sure_before + tie_before;
+        uint32_t at = sure_before;
         PGC_EACH_KEY {
-            const bool keep = key[j] >= tie_lo;
+            const bool keep = key[j] >= lo;
             const uint32_t m = __ballot_sync(0xffffffffu, keep);
             if (keep) {
                 const uint32_t o = at + __popc(m & lt);
@@ -259,7 +327,7 @@ __global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_
         }
     } else {
         PGC_EACH_KEY {
-            const bool sure = key[j] > tie_lo + tie_width, tie = key[j] - tie_lo <= tie_width;
+            const bool sure = key[j] > lo + width, tie = key[j] - lo <= width;
             const uint32_t ms = __ballot_sync(0xffffffffu, sure), mt = __ballot_sync(0xffffffffu, tie);
             const uint32_t rank_t = tie_before + __popc(mt & lt);
             if (sure || (tie && rank_t < need)) {
@@ -272,6 +340,16 @@ __global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_
         }
     }
 #undef PGC_EACH_KEY
+    // the first and the last tokens of this CTA's share
+    const int t1 = min(L, t0 + per * kSelThreads);
+    for (int t = t0 + tid; t < min(t1, F); t += kSelThreads) {
+        kept[t] = t;
+        if (wo != nullptr) wo[t] = vals[t - t0];
+    }
+    for (int t = max(t0, last) + tid; t < t1; t += kSelThreads) {
+        kept[B - L + t] = t;
+        if (wo != nullptr) wo[B - L + t] = vals[t - t0];
+    }
     if (wo != nullptr)
         for (int i = B + (int)rank * kSelThreads + tid; i < L; i += (int)ctas * kSelThreads) wo[i] = 0.f;
     if (ctas > 1) cluster_sync();  // a peer may still read this CTA's counts
@@ -372,7 +450,7 @@ cudaError_t launch_evict_select(const float *weights, float *weights_out, int64_
     // leaves SMs free takes more CTAs, up to 8, down to kSplitPer weights a thread, below which the
     // cluster's barriers cost more than they save. A CTA a row that reads it from L2 for every round
     // instead took 146 us there, and 51 us for one sequence of 262144.
-    constexpr int kSplitPer = 8, kLongRow = 32768;
+    constexpr int kSplitPer = 8, kLongRow = 131072;
     static_assert(kLongRow <= 8 * 512 * kMaxPer, "512 threads must hold the shorter rows");
     int sms = 148, dev = 0;
     cudaGetDevice(&dev);
@@ -400,8 +478,12 @@ cudaError_t launch_evict_select(const float *weights, float *weights_out, int64_
         }
         if (dev >= 0 && dev < 64) attr_set[dev] = true;
     }
-    const auto kern = threads == 1024 ? variants[3].kern : variants[per <= 8 ? 0 : per <= 16 ? 1 : 2].kern;
-    const size_t smem = hist_bytes + (weights_out != nullptr ? (size_t)(per + 3) / 4 * 4 * threads * sizeof(float) : 0);
+    const Variant &v = variants[threads == 1024 ? 3 : per <= 8 ? 0 : per <= 16 ? 1 : 2];
+    // A row takes the fewest CTAs that hold it where the grid fills the device, so that the others leave
+    // at once and make room; else as many as have kSplitPer weights a thread.
+    p.share = threads * ((int64_t)batch * kNumKvHeads * ctas * threads > (int64_t)sms * 1024 ? v.per : kSplitPer);
+    const int held = std::max((per + 3) / 4 * 4, p.share / threads);  // weights a thread, at most
+    const size_t smem = hist_bytes + (weights_out != nullptr ? (size_t)held * threads * sizeof(float) : 0);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, kNumKvHeads, batch);
     cfg.blockDim = dim3(threads);
@@ -420,7 +502,7 @@ cudaError_t launch_evict_select(const float *weights, float *weights_out, int64_
 #else
     cfg.numAttrs = 1;
 #endif
-    return cudaLaunchKernelEx(&cfg, kern, p);
+    return cudaLaunchKernelEx(&cfg, v.kern, p);
 }
 
 cudaError_t launch_evict_compact(const uint16_t *k_src, const uint16_t *v_src, int64_t src_pages,
