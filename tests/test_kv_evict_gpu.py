@@ -89,6 +89,38 @@ def test_select_longest(cuda):
     check_select(w, lens, 8192, 4, 1024, run_select(cuda, w, lens, 8192, 4, 1024, moved=False))
 
 
+@pytest.mark.parametrize("kind", ["tail", "close", "odd"])
+@pytest.mark.parametrize("longest", [40000, 140000])
+def test_select_large_batch(cuda, kind, longest):
+    """More rows than the device holds at once: each row uses as many CTAs of its cluster as hold it."""
+    rng = np.random.default_rng(longest)
+    lens = [longest, 513] + [int(x) for x in np.exp(rng.uniform(np.log(100), np.log(longest), 40))]
+    w = weights(rng, len(lens), longest, kind)
+    for in_place in (False, True):
+        got = run_select(cuda, w, lens, 512, 4, 100, in_place=in_place)
+        check_select(w, lens, 512, 4, 100, got, in_place=in_place)
+    assert cuda.device_error() == (0, 0)
+
+
+@pytest.mark.parametrize("n", [255, 256, 257, 1000])
+def test_select_crowded_value(cuda, n):
+    """n distinct neighbouring values around the last one kept, beside others: the list of those that are
+    left, at its size and past it, with need at either end."""
+    rng = np.random.default_rng(n)
+    L = 5000
+    w = (2.0 + rng.random((4, NKV, L))).astype(np.float32)
+    w[:, :, 1000:4000] = 2.0 ** rng.uniform(-30, 0, (4, NKV, 3000))
+    crowd = np.float32(1.0) + np.arange(n, dtype=np.float32) * np.float32(2.0 ** -23)
+    for s in range(4):
+        for h in range(NKV):
+            w[s, h, rng.choice(np.arange(1000, 4000), n, replace=False)] = rng.permutation(crowd)
+    above = int((w[0, 0] >= 2).sum())
+    for extra in (1, n // 2, n - 1, n, n + 1):
+        lens = [L] * 4
+        check_select(w, lens, above + extra, 0, 0, run_select(cuda, w, lens, above + extra, 0, 0))
+    assert cuda.device_error() == (0, 0)
+
+
 def test_select_slots_and_lengths(cuda):
     """Slots of the caller's choice; a slot named twice or out of range, or a length past the bound,
     keeps nothing and is reported."""
