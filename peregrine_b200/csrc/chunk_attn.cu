@@ -11,7 +11,7 @@
 //   * up to PGC_MAX_QUERIES rows: chunk_split_kernel (mma.sync), bound by the K/V bytes (64 sequences of
 //     1024 to 32768 tokens, 2.1 GB: 323 us, 6.5 TB/s); with weights it leaves the scores in the
 //     workspace, 16 B per row, kv head and token beside 1 KiB of K and V, so that K is read once;
-//   * more rows: chunk_pair_kernel on the 5th-gen tensor cores (1600 tokens over 24576: 496 us, 1340
+//   * more rows: chunk_pair_kernel on the 5th-gen tensor cores (1600 tokens over 24576: 463 us, 1440
 //     TFLOP/s), and chunk_weights.cu for the weights.
 // In both, the line of all the batch's tiles is cut into equal consecutive shares, one per CTA (or
 // pair) of a fixed grid: lengths are on the device, and a grid by the host's bounds would be empty for
@@ -783,6 +783,25 @@ static_assert(PairSmem::kWalk % 8 == 0, "walk slot");
 static_assert(PairSmem::kBytes <= 232448, "pair shared memory exceeds the sm_100 limit");
 static_assert(PGC_CHUNK_MAX_BATCH * 8 <= kKSlots * kKHalf, "the schedule's scratch is the K ring");
 
+// A pair's walk takes the unit that its share's start cuts last: every other unit it begins at its first
+// key, and as the pairs run at one speed, those of one kv head then read the same keys at about the same
+// time, from L2. A chunk of 1600 over 24576 reads 240 MB from HBM that way; in the line's order it read
+// 940 MB, as many cycles but a lower clock under the power cap (496 us instead of 463).
+// `first` is where the share starts, `later` whether that unit is still to come.
+__device__ __forceinline__ bool pair_begin(const RaggedBatch &rag, Walk &w) {
+    if (w.t0 == 0 || walk_last<PairTiling>(w)) return false;
+    walk_next<PairTiling>(rag, w);
+    return true;
+}
+__device__ __forceinline__ bool pair_next(const RaggedBatch &rag, Walk &w, bool &later, const Walk *first) {
+    if (walk_next<PairTiling>(rag, w)) return true;
+    if (!later) return false;
+    later = false;
+    w = *first;
+    w.left = w.tiles + PairTiling::kOver - w.off;  // and no further
+    return true;
+}
+
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     chunk_pair_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                       const __grid_constant__ CUtensorMap tmv, const PairParams p) {
@@ -821,6 +840,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     // the record of the share, that no unit is cut by its end until its walk has ended
     if (leader && threadIdx.x == 0) p.frags[pair].last = p.frags[pair].first = 0;
     if (!busy) return;  // both CTAs of the pair
+    const Walk *first = reinterpret_cast<const Walk *>(smem + PairSmem::kWalk);
+    bool later = pair_begin(p.rag, w);
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         mbar_init(q_full, 2);
@@ -906,7 +927,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                             tma_load_2d_pair(dst + c * (64 * 128) + pp * 2048, &tmk, c * 64, row, kbar, pol);
                     }
                 }
-                if (!walk_next<PairTiling>(p.rag, w)) break;
+                if (!pair_next(p.rag, w, later, first)) break;
             }
         }
     } else if (warp >= kSoftmaxWarps + 1 + kProducerWarps) {
@@ -973,7 +994,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 }
                 __syncwarp();
             }
-            if (!walk_next<PairTiling>(p.rag, w)) break;
+            if (!pair_next(p.rag, w, later, first)) break;
         }
     } else if (warp == kSoftmaxWarps) {
         // ------------------------------------------------------------ pair MMA issuer (leader)
@@ -990,7 +1011,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             // for that unit's Q to be replaced.
             Walk a = w;
             int at = a.t0, ag = 0, aunit = 0;
-            bool more = true, ok = true;
+            bool more = true, ok = true, alater = later;
             auto issue_s = [&]() -> bool {
                 const int b = ag & 1, sl = ag % kKSlots;
                 if (at == a.t0 && !wait(q_full, aunit & 1, 4)) return false;
@@ -1006,7 +1027,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 ++ag;
                 if (++at == a.t1) {
                     umma2_commit_pair_elected(me, q_empty);
-                    more = walk_next<PairTiling>(p.rag, a);
+                    more = pair_next(p.rag, a, alater, first);
                     at = a.t0;
                     ++aunit;
                 }
@@ -1035,7 +1056,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     umma2_commit_pair_elected(me, &v_empty[sl]);
                     umma2_commit_pair_elected(me, &pv_done[b]);
                 }
-                if (!ok || !walk_next<PairTiling>(p.rag, w)) break;
+                if (!ok || !pair_next(p.rag, w, later, first)) break;
             }
         }
     } else {
@@ -1194,11 +1215,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 for (int i = 0; i < 32; i += 4)
                     *reinterpret_cast<uint4 *>(dst + 2 * i) = make_uint4(ow[i], ow[i + 1], ow[i + 2], ow[i + 3]);
             }
-            if (walk_last<PairTiling>(w)) {
-                if (leader && threadIdx.x == 0 && w.t0 == 0) write_record<PairTiling>(&p.frags[pair], w, *line, pair);
-                break;
-            }
-            walk_next<PairTiling>(p.rag, w);
+            if (leader && threadIdx.x == 0 && w.t0 == 0 && walk_last<PairTiling>(w))
+                write_record<PairTiling>(&p.frags[pair], w, *line, pair);
+            if (!pair_next(p.rag, w, later, first)) break;
         }
     }
     // neither CTA may leave (or free TMEM) while the pair MMA or the peer can still touch it
