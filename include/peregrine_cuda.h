@@ -277,7 +277,8 @@ size_t pgc_chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_
  * A masked token's score is never used, whatever it is, and slots past a sequence's end are never
  * read into a sum; but a NaN or infinite V element of a cached token of the sequence makes that output
  * dim NaN in rows before the token too (its probability there is 0, and 0 times it is NaN).
- * q, k/v_pages, gate, out and workspace 16-byte aligned; out, lse and the workspace overlap no input.
+ * q, k/v_pages, gate, out and workspace 16-byte aligned, the other arrays to their elements; out, lse and
+ * the workspace overlap no input.
  * Calls that may overlap on the GPU, and graphs that may, need workspaces of their own. The work is
  * dealt out by the whole batch's lengths: the same batch gives the same bits every time, a sequence
  * in another batch the same values within rounding. */
@@ -323,7 +324,7 @@ int pgc_chunk_attn_weights(const uint16_t *q, const uint16_t *k_pages, const uin
  *   kept         [batch][4][budget] int32: the kept indices, ascending; -1 behind the last
  *   new_lens     nullable [batch] int32: min(L, budget); not seq_lens itself
  * A length outside [0, max_seq_len], or a slot that may not be used, is recorded and the sequence
- * keeps nothing (kept -1, new_lens 0). budget >= 1, keep_first + keep_last <= budget,
+ * keeps nothing (kept -1, new_lens 0). 1 <= budget <= 2^30, keep_first + keep_last <= budget,
  * max_seq_len <= PGC_EVICT_MAX_TOKENS, batch <= 65535. */
 int pgc_kv_evict_select(const float *weights, float *weights_out, int64_t weights_stride,
                         int64_t num_slots, const int32_t *slots, const int32_t *seq_lens, int batch,

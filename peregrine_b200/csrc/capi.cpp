@@ -80,6 +80,7 @@ int check_device(int *dev_out) {
 }
 
 inline bool al16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
+inline bool al4(const void *p) { return ((uintptr_t)p & 3u) == 0; }
 
 int cuda_status(cudaError_t e) { return e == cudaSuccess ? PGC_OK : PGC_ERR_CUDA; }
 
@@ -514,7 +515,8 @@ static int chunk_call(const uint16_t *q, const uint16_t *k_pages, const uint16_t
     if (num_pages * 4 * 16 > INT32_MAX) return PGC_ERR_BOUNDS;  // TMA row coordinate is int32
     if (total_q > PGC_CHUNK_MAX_ROWS || max_seq_len > PGC_CHUNK_MAX_TOKENS) return PGC_ERR_BOUNDS;
     if (!al16(q) || !al16(k_pages) || !al16(v_pages) || !al16(gate) || !al16(out) || !al16(workspace) ||
-        ((uintptr_t)lse & 3u) != 0 || (weights && ((uintptr_t)weights->weights & 3u) != 0))
+        !al4(block_tables) || !al4(q_starts) || !al4(seq_lens) || !al4(lse) ||
+        (weights && (!al4(weights->weights) || !al4(weights->slots))))
         return PGC_ERR_ALIGN;
     const int sms = current_sm_count();
     if (!workspace || workspace_bytes < chunk_workspace_bytes(batch, total_q, max_q_len, max_seq_len,
@@ -570,12 +572,13 @@ int pgc_kv_evict_select(const float *weights, float *weights_out, int64_t weight
     if (batch < 0 || max_seq_len < 0 || num_slots <= 0 || budget < 1 || keep_first < 0 || keep_last < 0 ||
         (int64_t)keep_first + keep_last > budget)
         return PGC_ERR_INVALID;
-    if (batch > 65535 || max_seq_len > PGC_EVICT_MAX_TOKENS || weights_stride < max_seq_len ||
+    if (batch > 65535 || max_seq_len > PGC_EVICT_MAX_TOKENS || budget > (1 << 30) || weights_stride < max_seq_len ||
         (!slots && batch > num_slots))
         return PGC_ERR_BOUNDS;
     if (batch == 0) return PGC_OK;
     if (!weights || !seq_lens || !kept || new_lens == seq_lens) return PGC_ERR_INVALID;
-    if (((uintptr_t)weights & 3u) != 0 || ((uintptr_t)weights_out & 3u) != 0) return PGC_ERR_ALIGN;
+    if (!al4(weights) || !al4(weights_out) || !al4(slots) || !al4(seq_lens) || !al4(kept) || !al4(new_lens))
+        return PGC_ERR_ALIGN;
     const int st = check_device(nullptr);
     if (st != PGC_OK) return st;
     return cuda_status(launch_evict_select(weights, weights_out, weights_stride, num_slots, slots, seq_lens, batch,
@@ -594,7 +597,9 @@ int pgc_kv_evict_compact(const uint16_t *src_k_pages, const uint16_t *src_v_page
         return PGC_ERR_INVALID;
     if ((int64_t)dst_max_pages * PGC_PAGE_TOKENS < budget) return PGC_ERR_BOUNDS;
     if ((int64_t)batch * budget > INT32_MAX / 4) return PGC_ERR_BOUNDS;  // rows, the grid
-    if (!al16(src_k_pages) || !al16(src_v_pages) || !al16(dst_k_pages) || !al16(dst_v_pages)) return PGC_ERR_ALIGN;
+    if (!al16(src_k_pages) || !al16(src_v_pages) || !al16(dst_k_pages) || !al16(dst_v_pages) || !al4(src_tables) ||
+        !al4(kept) || !al4(dst_tables))
+        return PGC_ERR_ALIGN;
     const int st = check_device(nullptr);
     if (st != PGC_OK) return st;
     return cuda_status(launch_evict_compact(src_k_pages, src_v_pages, src_num_pages, src_tables, src_max_pages, kept,

@@ -98,3 +98,18 @@ COMPACT = dict(k=A, v=A, pages=100, tables=A, width=10, kept=A, batch=2, budget=
     (dict(dv=A + 2), ALIGN), (dict(batch=0), 0), (dict(budget=0), 0)])
 def test_compact_refusals(lib, change, status):
     assert lib.pgc_kv_evict_compact(*{**COMPACT, **change}.values()) == status
+
+
+def test_index_arrays_must_be_aligned(lib):
+    for name in ("tables", "starts", "lens"):
+        for weights in (False, True):
+            assert chunk(lib, weights, **{name: A + 2}) == ALIGN
+    assert chunk(lib, True, slots=A + 1) == ALIGN
+    for name in ("slots", "lens", "kept", "new"):
+        assert lib.pgc_kv_evict_select(*{**SELECT, name: A + 2}.values()) == ALIGN
+    for name in ("tables", "kept", "dtables"):
+        assert lib.pgc_kv_evict_compact(*{**COMPACT, name: A + 1}.values()) == ALIGN
+
+
+def test_select_budget_bound(lib):
+    assert lib.pgc_kv_evict_select(*{**SELECT, "budget": (1 << 30) + 1}.values()) == BOUNDS
