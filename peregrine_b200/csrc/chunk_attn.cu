@@ -22,6 +22,8 @@
 // the first load, 4 to 6 of loads, 2 for the join in the CTA, 5 for the second kernel.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "pgc_common.cuh"
 #include "pgc_internal.h"
 #include "pgc_ragged.cuh"
@@ -289,10 +291,6 @@ __device__ __forceinline__ void write_record(Fragment *f, const Walk &w, const L
 // ring run on from unit to unit, Q is double-buffered, so only the end of the share drains.
 // Two CTAs an SM (register-bound) keep 128 KiB of pages in flight.
 // =============================================================================================
-constexpr int kConsumers = 4;
-constexpr int kSplitThreads = (kConsumers + 1) * 32;
-constexpr int kStages = 4;
-static_assert(kStages % kConsumers == 0, "each stage must belong to one consumer warp");
 constexpr int kTileBytes = kPage * kHeadDim * 2;  // one (page, kv head) of K or V: 8 KiB
 constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kRows = PGC_MAX_QUERIES * kGroup;
@@ -313,24 +311,36 @@ struct SplitParams {
     float *scores;     // nullable: [total_q][4][score_stride][4], scaled by log2(e)
     int64_t score_stride;
     float scale_log2;
+    int cluster;  // CTAs of a cluster, in the cluster form
+    ChunkWeights w;
 };
 
+constexpr int kConsumers = 4;
+template <int kStagesOf, int kProducersOf>
 struct SplitSmem {
+    static constexpr int kStages = kStagesOf, kProducers = kProducersOf;
+    static constexpr int kThreads = (kConsumers + kProducers) * 32;
     static constexpr int kRing = 0;  // 1024-aligned
     static constexpr int kQ = kRing + kStages * kStageBytes;
     static constexpr int kJoin = kQ + 2 * kRows * kQRowBytes;
     static constexpr int kM = kJoin + kConsumers * 4 * kJoinPitch * 4;  // [4 warps][16 rows]
     static constexpr int kL = kM + kConsumers * kRows * 4;
-    static constexpr int kBar = kL + kConsumers * kRows * 4;  // full[4], empty[4], q_full[2], q_empty[2]
+    static constexpr int kBar = kL + kConsumers * kRows * 4;  // full[stages], empty[stages], q_full[2], q_empty[2]
     static constexpr int kWalk = kBar + (2 * kStages + 4) * 8;  // per consumer warp
     static constexpr int kLine = kWalk + kConsumers * sizeof(Walk);
     static constexpr int kAbort = kLine + 24;
     static constexpr int kBytes = kAbort + 8;
+    static constexpr int kAlloc = kBytes + 1024;  // + alignment slack
+    static_assert(kStages % kConsumers == 0, "each stage must belong to one consumer warp");
+    static_assert(sizeof(Walk) <= 48 && sizeof(Line) <= 24 && kWalk % 8 == 0, "schedule slots");
+    static_assert(PGC_CHUNK_MAX_BATCH * 8 <= kStages * kStageBytes, "the schedule's scratch is the ring");
+    static_assert(kConsumers * kRows * kJoinPitch * 4 <= kJoin, "the last join's scratch is the ring and Q");
+    static_assert(kRows * kHeadDim * 4 <= kM - kJoin, "the cluster's exchange is the join's scratch");
 };
-constexpr int kSplitSmem = SplitSmem::kBytes + 1024;  // + alignment slack
-static_assert(sizeof(Walk) <= 48 && sizeof(Line) <= 24 && SplitSmem::kWalk % 8 == 0, "schedule slots");
-static_assert(PGC_CHUNK_MAX_BATCH * 8 <= kStages * kStageBytes, "the schedule's scratch is the ring");
-static_assert(kConsumers * kRows * kJoinPitch * 4 <= SplitSmem::kJoin, "the last join's scratch is the ring and Q");
+constexpr int kMaxCluster = 16;
+using LineSmem = SplitSmem<4, 1>;     // two CTAs an SM
+using ClusterSmem = SplitSmem<8, 4>;  // one CTA an SM
+static_assert(2 * ClusterSmem::kAlloc > 227 * 1024, "a cluster's CTAs are to have an SM each");
 
 // Untiled bulk copy global -> shared, completion bytes on `bar`; 16-byte aligned, a multiple of 16.
 __device__ __forceinline__ void bulk_load(void *smem_dst, const void *src, uint32_t bytes, uint64_t *bar) {
@@ -354,10 +364,128 @@ __device__ __forceinline__ void tma_load_page(void *smem_dst, const void *tmap, 
         : "memory");
 }
 
-template <bool kScores>
-__global__ void __launch_bounds__(kSplitThreads, 2)
+// Two floats of another CTA's shared memory, at this CTA's address of them.
+__device__ __forceinline__ float2 load_peer2(const void *at, uint32_t rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_map(smem_u32(at), rank)) : "memory");
+    return v;
+}
+
+// The end of the cluster form's one unit. Every consumer warp has its part of O in `o` (on m_s, with
+// c0 and c1 to the CTA's common maximum) and the parts of the sums in l_s. The CTA adds its warps' up into
+// `part` ([16 rows][256] and the rows' maximum and sum), and CTA `rank` joins 256 / ctas dims of all rows
+// from the cluster's parts, in the CTAs' order. With scores it then adds its own tokens' weights.
+template <bool kScores, class Sync>
+__device__ __forceinline__ void join_cluster(const SplitParams &p, uint8_t *ring, uint8_t *scratch, float *m_s, float *l_s,
+                                             const Walk &w, const float (&o)[32][4], float c0, float c1, int ctas, int rank,
+                                             const Sync &sync) {
+    __shared__ float2 stat[kRows];                // m (log2 units) and l of this CTA, read by the cluster
+    __shared__ float2 stats[kRows][kMaxCluster];  // of all
+    __shared__ __align__(16) float lse2[kRows];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int r0 = lane >> 2, cpair = (lane & 3) * 2, nrows = w.n * kGroup;
+    float *buf = reinterpret_cast<float *>(ring), *part = reinterpret_cast<float *>(scratch);
+    constexpr int kThreads = kConsumers * 32;
+    const int jrows = nrows <= 4 ? 4 : nrows <= 8 ? 8 : 16;
+    float *to = buf + (warp * jrows + r0) * kJoinPitch + cpair;
+    if (r0 < nrows) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) *reinterpret_cast<float2 *>(to + i * 8) = make_float2(o[i][0] * c0, o[i][1] * c0);
+    }
+    if (r0 + 8 < nrows) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) *reinterpret_cast<float2 *>(to + 8 * kJoinPitch + i * 8) = make_float2(o[i][2] * c1, o[i][3] * c1);
+    }
+    sync();
+    const int dim = tid % (kHeadDim / 2) * 2;
+    for (int r = tid / (kHeadDim / 2); r < nrows; r += kThreads / (kHeadDim / 2)) {
+        float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < kConsumers; ++q)
+            acc = __fadd2_rn(acc, *reinterpret_cast<const float2 *>(&buf[(q * jrows + r) * kJoinPitch + dim]));
+        *reinterpret_cast<float2 *>(&part[r * kHeadDim + dim]) = acc;
+    }
+    if (tid < nrows) {
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int q = 0; q < kConsumers; ++q) {
+            m = fmaxf(m, m_s[q * kRows + tid]);
+            l += l_s[q * kRows + tid];
+        }
+        stat[tid] = make_float2(m, l);
+    }
+    const int pairs = kHeadDim / 2 / ctas;  // of dims, of every row: this CTA's part of the join
+    auto out_row = [&](int r) { return (int64_t)(w.row0 + r / kGroup) * kNumQHeads + w.kvh * kGroup + r % kGroup; };
+    auto load_gate = [&](int e) -> uint32_t {
+        if (p.gate == nullptr || e >= nrows * pairs) return 0;
+        return *reinterpret_cast<const uint32_t *>(p.gate + out_row(e / pairs) * kHeadDim + (rank * pairs + e % pairs) * 2);
+    };
+    uint32_t gv = load_gate(tid);  // ahead of the barriers
+    cluster_sync_all();
+    for (int i = tid; i < nrows * ctas; i += kThreads) stats[i / ctas][i % ctas] = load_peer2(&stat[i / ctas], i % ctas);
+    sync();
+    for (int e = tid; e < nrows * pairs; e += kThreads) {
+        const int r = e / pairs, d = (rank * pairs + e % pairs) * 2;
+        float2 v[kMaxCluster];
+#pragma unroll
+        for (int q = 0; q < kMaxCluster; ++q)
+            if (q < ctas) v[q] = load_peer2(&part[r * kHeadDim + d], q);
+        const uint32_t g = gv;
+        gv = load_gate(e + kThreads);
+        float mx = -INFINITY;
+        for (int q = 0; q < ctas; ++q) mx = fmaxf(mx, stats[r][q].x);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        float den = 0.f;
+        float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < kMaxCluster; ++q) {
+            if (q >= ctas) break;
+            const float c = fast_exp2(stats[r][q].x - base);
+            den += stats[r][q].y * c;
+            acc.x += v[q].x * c;
+            acc.y += v[q].y * c;
+        }
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        acc.x *= inv;
+        acc.y *= inv;
+        if (p.gate != nullptr) {
+            acc.x = sigmoid_gate(acc.x, g & 0xffffu);
+            acc.y = sigmoid_gate(acc.y, g >> 16);
+        }
+        *reinterpret_cast<uint32_t *>(p.out + out_row(r) * kHeadDim + d) = pack_bf16x2(acc.x, acc.y);
+        if (e % pairs == 0) {
+            // +inf for a row whose sum is 0, so that its -inf scores add nothing
+            if (kScores) lse2[r] = den == 0.f ? INFINITY : mx + log2f(den);
+            if (rank == 0 && p.lse != nullptr) p.lse[out_row(r)] = den == 0.f ? -INFINITY : mx * kLn2 + logf(den);
+        }
+    }
+    if (kScores) {
+        sync();  // also this CTA's scores are all written
+        const int64_t slot = ragged_slot(p.w.slots, p.w.num_slots, w.seq, w.kvh == 0 && rank == 0 && warp == 0 ? &g_chunk_err : nullptr);
+        if (slot >= 0) {
+            float *wt = p.w.weights + (slot * kNumKvHeads + w.kvh) * p.w.stride;
+            const float4 *s = reinterpret_cast<const float4 *>(p.scores) + ((int64_t)w.row0 * kNumKvHeads + w.kvh) * p.score_stride;
+            const int end = min(w.len, w.t1 * kPage);
+            for (int t = w.t0 * kPage + tid; t < end; t += kThreads) {
+                float sum = wt[t];
+                for (int j = max(0, t - (w.len - w.n)); j < w.n; ++j) {  // the rows that see it
+                    const float4 x = s[(int64_t)j * kNumKvHeads * p.score_stride + t];
+                    const float4 l = *reinterpret_cast<const float4 *>(&lse2[j * kGroup]);
+                    sum += (fast_exp2(x.x - l.x) + fast_exp2(x.y - l.y)) + (fast_exp2(x.z - l.z) + fast_exp2(x.w - l.w));
+                }
+                wt[t] = sum;
+            }
+        }
+    }
+    cluster_sync_all();  // peers may still read this CTA's part
+}
+
+template <bool kScores, bool kCluster>
+__global__ void __launch_bounds__(kCluster ? ClusterSmem::kThreads : LineSmem::kThreads, kCluster ? 1 : 2)
     chunk_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                        const SplitParams p) {
+    using SplitSmem = std::conditional_t<kCluster, ClusterSmem, LineSmem>;
+    constexpr int kStages = SplitSmem::kStages, kProducers = SplitSmem::kProducers;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + SplitSmem::kBar);
@@ -377,7 +505,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], kProducers == 1 ? 1 : 2);
             mbar_init(&empty[s], 1);
         }
         for (int s = 0; s < 2; ++s) {
@@ -390,21 +518,40 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     }
     pdl_wait();
     Walk w;
-    const bool busy = find_share<SplitTiling>(p.rag, reinterpret_cast<int64_t *>(smem + SplitSmem::kRing), index,
-                                              gridDim.x, reinterpret_cast<Walk *>(smem + SplitSmem::kWalk), line,
-                                              index == 0 ? &g_chunk_err : nullptr, w);
-    if (!busy) return;
-    fence_proxy_async_smem();  // the schedule's scratch becomes the ring
+    const int ctas = p.cluster, rank = kCluster ? index % ctas : 0;
+    if constexpr (kCluster) {
+        const int unit = index / ctas;
+        w.seq = unit / kNumKvHeads;
+        w.kvh = unit % kNumKvHeads;
+        w.qt = 0;
+        const RaggedSeq s = ragged_seq(p.rag, w.seq, unit % kNumKvHeads + rank + threadIdx.x == 0 ? &g_chunk_err : nullptr);
+        if (s.n == 0) return;  // the whole cluster
+        w.row0 = s.row0;
+        w.n = s.n;
+        w.len = s.len;
+        w.tiles = unit_tiles<SplitTiling>(w.n, w.len, 0);
+        w.t0 = (int)((int64_t)w.tiles * rank / ctas);
+        w.t1 = (int)((int64_t)w.tiles * (rank + 1) / ctas);
+        w.off = w.left = 0;  // nothing behind it
+    } else {
+        const bool busy = find_share<SplitTiling>(p.rag, reinterpret_cast<int64_t *>(smem + SplitSmem::kRing), index,
+                                                  gridDim.x, reinterpret_cast<Walk *>(smem + SplitSmem::kWalk), line,
+                                                  index == 0 ? &g_chunk_err : nullptr, w);
+        if (!busy) return;
+        fence_proxy_async_smem();  // the schedule's scratch becomes the ring
+    }
     __syncthreads();
 
-    if (warp == kConsumers) {
-        // ------------------------------------------------------------ producer
+    if (warp >= kConsumers) {
+        // ------------------------------------------------------------ producers
+        // one for all, or of four: K or V (bit 0), of every second tile (bit 1)
+        const int pw = warp - kConsumers;
         const uint64_t pol = l2_policy_evict_first();
         int g = 0;
         for (int unit = 0;; ++unit) {
             const int qb = unit & 1;
             bool ok = true;
-            if (lane == 0) {
+            if (lane == 0 && pw == kProducers - 1) {
                 ok = unit < 2 || wait(&q_empty[qb], ((unit >> 1) - 1) & 1, 21);
                 if (ok) {
                     mbar_arrive_expect_tx(&q_full[qb], (uint32_t)w.n * kGroup * kHeadDim * 2);
@@ -430,23 +577,23 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
                     }
                 }
                 const int page = __shfl_sync(0xffffffffu, ids, k);
-                if (lane == 0) {
+                if (lane == 0 && (kProducers == 1 || (g & 1) == pw >> 1)) {
                     const int s = g % kStages, round = g / kStages;
                     if (round > 0 && !wait(&empty[s], (round - 1) & 1, 22)) {
                         ok = false;
                     } else if (t * kPage < w.len) {
                         uint8_t *stage = smem + SplitSmem::kRing + s * kStageBytes;
-                        mbar_arrive_expect_tx(&full[s], kStageBytes);
+                        mbar_arrive_expect_tx(&full[s], kProducers == 1 ? kStageBytes : kTileBytes);
                         const int row = (page * kNumKvHeads + w.kvh) * kPage;
-                        tma_load_page(stage, &tmk, row, &full[s], pol);
-                        tma_load_page(stage + kTileBytes, &tmv, row, &full[s], pol);
+                        if (kProducers == 1 || (pw & 1) == 0) tma_load_page(stage, &tmk, row, &full[s], pol);
+                        if (kProducers == 1 || (pw & 1) == 1) tma_load_page(stage + kTileBytes, &tmv, row, &full[s], pol);
                     } else {
                         mbar_arrive(&full[s]);  // an empty cache: the tile is all masked
                     }
                 }
                 ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0);
             }
-            if (!ok || !walk_next<SplitTiling>(p.rag, w)) break;
+            if (!ok || kCluster || !walk_next<SplitTiling>(p.rag, w)) break;
         }
         return;
     }
@@ -620,6 +767,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         if ((lane & 3) == 0) {
             l_s[warp * kRows + r0] = l0 * c0;
             l_s[warp * kRows + r0 + 8] = l1 * c1;
+        }
+        if constexpr (kCluster) {
+            join_cluster<kScores>(p, smem, smem + SplitSmem::kJoin, m_s, l_s, *ws, o, c0, c1, ctas, rank, sync);
+            return;
         }
         Walk w = *ws;
         const bool whole = w.t0 == 0 && w.t1 == w.tiles;
@@ -1427,7 +1578,7 @@ __device__ __forceinline__ void merge_row(const FinishParams &p, const Fragment 
 // the rows' lse: the split kernel's, or for a cut unit formed from the fragments' (m, l) here, so that
 // these blocks need not wait for the merging ones.
 __device__ __forceinline__ void add_weights(const FinishParams &p, int blk) {
-    __shared__ float lse2[kRows];  // log2 units
+    __shared__ __align__(16) float lse2[kRows];  // log2 units
     const int chunk = blk % p.add_chunks, unit = blk / p.add_chunks;
     const int kvh = unit % kNumKvHeads, b = unit / kNumKvHeads;
     const Fragment f = read_record(p, unit);  // of a sequence with rows only
@@ -1518,6 +1669,51 @@ __global__ void __launch_bounds__(kFinishThreads) chunk_finish_kernel(const Fini
     }
 }
 
+// The split form's cluster form: its launch, and the CTAs of a cluster (0: the line form is to be taken). A
+// short batch is bound by latency, which the cluster form has less of (one launch); but it takes the
+// sequences as they are, so it is for batches whose clusters all run at once, and up to kClusterTokens a
+// CTA. One row, us: 500 tokens 7.0 against 12.8 of the line form, 4097 10.6 against 15.8, 16000 21.5 against
+// 22.5, 32768 36.8 against 33.1; 8 sequences of 1000 9.9 against 15.7, 37 of 300 13.5 against 21.2. Where the
+// clusters took two turns: 4 sequences of 300, 8 CTAs each, 11.9 against 12.9, of 2000 16.3 against 16.2.
+constexpr int kClusterTokens = 512;
+struct ClusterLaunch {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    ClusterLaunch(int clusters, int ctas, cudaStream_t stream) {
+        cfg.gridDim = dim3(clusters * ctas);
+        cfg.blockDim = dim3(ClusterSmem::kThreads);
+        cfg.dynamicSmemBytes = ClusterSmem::kAlloc;
+        cfg.stream = stream;
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ctas;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+#ifndef PGC_NO_PDL
+        cfg.numAttrs = 2;
+#else
+        cfg.numAttrs = 1;
+#endif
+    }
+};
+inline int cluster_of(int dev, int batch, int max_seq_len) {
+    static std::atomic<int> held[64][5] = {};  // clusters of 1 << k CTAs that run at once, + 1
+    for (int k = 4; k >= 0; --k) {
+        int n = dev >= 0 && dev < 64 ? held[dev][k].load() - 1 : -1;
+        if (n < 0) {
+            ClusterLaunch l(1, 1 << k, nullptr);
+            if (cudaOccupancyMaxActiveClusters(&n, chunk_split_kernel<true, true>, &l.cfg) != cudaSuccess) {
+                cudaGetLastError();
+                n = 0;
+            }
+            if (dev >= 0 && dev < 64) held[dev][k] = n + 1;
+        }
+        if (batch * kNumKvHeads <= n) return max_seq_len <= kClusterTokens << k ? 1 << k : 0;
+    }
+    return 0;
+}
+
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Workspace of a call: the shares' records and partials, with weights the rows' lse, and in the split
@@ -1560,8 +1756,12 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
     if (dev < 0 || dev >= 64 || !attr_set[dev]) {
         const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
         cudaError_t e = cudaFuncSetAttribute(chunk_pair_kernel, attr, PairSmem::kBytes);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_split_kernel<false>, attr, kSplitSmem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_split_kernel<true>, attr, kSplitSmem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_split_kernel<false, false>, attr, LineSmem::kAlloc);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_split_kernel<true, false>, attr, LineSmem::kAlloc);
+        for (auto kern : {chunk_split_kernel<false, true>, chunk_split_kernel<true, true>}) {
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, attr, ClusterSmem::kAlloc);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        }
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) attr_set[dev] = true;
     }
@@ -1591,9 +1791,15 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
         sp.scores = weights != nullptr ? reinterpret_cast<float *>(ws + lay.scores) : nullptr;
         sp.score_stride = lay.score_stride;
         sp.scale_log2 = scale * kLog2e;
-        const dim3 grid(lay.shares), block(kSplitThreads);
-        cudaError_t e = weights != nullptr ? launch_pdl(chunk_split_kernel<true>, grid, block, kSplitSmem, stream, tk, tv, sp)
-                                           : launch_pdl(chunk_split_kernel<false>, grid, block, kSplitSmem, stream, tk, tv, sp);
+        sp.cluster = cluster_of(dev, rag.batch, rag.max_seq_len);
+        if (sp.cluster != 0) {
+            if (weights != nullptr) sp.w = *weights;
+            ClusterLaunch l(rag.batch * kNumKvHeads, sp.cluster, stream);
+            return cudaLaunchKernelEx(&l.cfg, weights != nullptr ? chunk_split_kernel<true, true> : chunk_split_kernel<false, true>, tk, tv, sp);
+        }
+        const dim3 grid(lay.shares), block(LineSmem::kThreads);
+        cudaError_t e = weights != nullptr ? launch_pdl(chunk_split_kernel<true, false>, grid, block, LineSmem::kAlloc, stream, tk, tv, sp)
+                                           : launch_pdl(chunk_split_kernel<false, false>, grid, block, LineSmem::kAlloc, stream, tk, tv, sp);
         if (e != cudaSuccess) return e;
         fp.rag = rag;
         // a few hundred blocks cover the records: most of a large batch's are of units not cut
