@@ -280,8 +280,9 @@ size_t pgc_chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_
  * q, k/v_pages, gate, out and workspace 16-byte aligned, the other arrays to their elements; out, lse and
  * the workspace overlap no input.
  * Calls that may overlap on the GPU, and graphs that may, need workspaces of their own. The work is
- * dealt out by the whole batch's lengths: the same batch gives the same bits every time, a sequence
- * in another batch the same values within rounding. */
+ * dealt out by the whole batch's lengths, and its form chosen by batch, max_q_len and max_seq_len: the
+ * same call gives the same bits every time, a sequence in another batch, or under other bounds, the same
+ * values within rounding. */
 int pgc_chunk_attn(const uint16_t *q, const uint16_t *k_pages, const uint16_t *v_pages,
                    int64_t num_pages, const int32_t *block_tables, int max_pages_per_seq,
                    const int32_t *q_starts, const int32_t *seq_lens, int batch, int total_q,

@@ -7,19 +7,19 @@
 // and, with weights, w[kv head][t] += sum over the kv head's 4 query heads and the rows of
 // exp(s_t - lse). A row that sees nothing (p < 0) has o = 0 and lse = -inf.
 //
-// Two forms, chosen by the host bound on the rows of a sequence:
-//   * up to PGC_MAX_QUERIES rows: chunk_split_kernel (mma.sync), bound by the K/V bytes (64 sequences of
-//     1024 to 32768 tokens, 2.1 GB: 323 us, 6.5 TB/s); with weights it leaves the scores in the
-//     workspace, 16 B per row, kv head and token beside 1 KiB of K and V, so that K is read once;
+// Forms, chosen by the host bounds:
+//   * up to PGC_MAX_QUERIES rows a sequence: chunk_split_kernel (mma.sync), bound by the K/V bytes (64
+//     sequences of 1024 to 32768 tokens, 2.1 GB: 323 us, 6.5 TB/s); with weights it leaves the scores in
+//     the workspace, 16 B per row, kv head and token beside 1 KiB of K and V, so that K is read once.
+//     Few short sequences take its cluster form, bound by latency (one row over 4097 tokens: 10.7 us,
+//     over 500: 7.0);
 //   * more rows: chunk_pair_kernel on the 5th-gen tensor cores (1600 tokens over 24576: 463 us, 1440
 //     TFLOP/s), and chunk_weights.cu for the weights.
-// In both, the line of all the batch's tiles is cut into equal consecutive shares, one per CTA (or
-// pair) of a fixed grid: lengths are on the device, and a grid by the host's bounds would be empty for
-// the most part where they are ragged (387 us for the 64 sequences above). A unit of work cut by a
-// share's border leaves fp32 partials, at most two units a share (its first and its last), which a
+// But for the cluster form, the line of all the batch's tiles is cut into equal consecutive shares, one
+// per CTA (or pair) of a fixed grid: lengths are on the device, and a grid by the host's bounds would be
+// empty for the most part where they are ragged (387 us for the 64 sequences above). A unit of work cut by
+// a share's border leaves fp32 partials, at most two units a share (its first and its last), which a
 // second kernel joins; every other unit is written where it is computed.
-// One-row calls of one or a few sequences are bound by latency, about 16 us for 4097 tokens: 2 us to
-// the first load, 4 to 6 of loads, 2 for the join in the CTA, 5 for the second kernel.
 #include <cuda.h>
 
 #include <type_traits>
@@ -290,6 +290,11 @@ __device__ __forceinline__ void write_record(Fragment *f, const Walk &w, const L
 // tensor pipe is mostly idle (a kv head has 4 to 16 query rows): HBM bounds it. The producer and the
 // ring run on from unit to unit, Q is double-buffered, so only the end of the share drains.
 // Two CTAs an SM (register-bound) keep 128 KiB of pages in flight.
+// In the cluster form (kCluster) a cluster of CTAs has one unit, its pages split evenly in order, and joins
+// through distributed shared memory: no shares to find, no partials in memory, no second launch. A CTA has
+// an SM to itself, and one issuing warp's TMA delivers only about 21 B a cycle to an SM: four producer
+// warps (K or V, of every second page) took one row over 4097 tokens from 11.8 to 10.7 us, over 16000 from
+// 26.1 to 21.5. Eight consumer warps instead of four made it slower (12.8).
 // =============================================================================================
 constexpr int kTileBytes = kPage * kHeadDim * 2;  // one (page, kv head) of K or V: 8 KiB
 constexpr int kStageBytes = 2 * kTileBytes;

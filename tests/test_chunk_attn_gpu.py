@@ -260,3 +260,77 @@ def test_long_cache_offsets(cuda):
     got = call(cuda, dict(c, k=k, v=v, tables=tables))
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert cuda.device_error() == (0, 0)
+
+
+def in_line_form(c, lmax=40000):
+    """The batch with a host bound that no cluster takes: units cut over the whole grid, joined by a second
+    kernel. (Short batches within the bounds run as a cluster per sequence and kv head.)"""
+    import torch
+    width = -(-lmax // 16)
+    return dict(c, lmax=lmax, tables=torch.nn.functional.pad(c["tables"], (0, width - c["tables"].shape[1]), value=1 << 30))
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("name", [n for n in SMALL if len(SMALL[n]) < 100])
+def test_short_batches_in_line_form(cuda, name, weights):
+    import torch
+    c = in_line_form(make(SMALL[name], seed=20 + len(name), first_row=1, rows_behind=2, gate=len(name) % 2 == 1))
+    w = before = None
+    if weights:
+        before = torch.rand((len(SMALL[name]), NKV, c["lmax"]), device="cuda")
+        w = before.clone()
+    got = call(cuda, c, weights=w)
+    torch.cuda.synchronize()
+    assert cuda.device_error() == (0, 0)
+    check(c, got, reference(c), w, before)
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("batch", [1, 2, 3, 4, 7, 8, 9, 18, 19, 36, 37, 38])
+def test_batch_sizes(cuda, batch, weights):
+    """Every cluster size, its edges in the number of sequences, and lengths from none to the longest that
+    it takes and one more; rows from none to 4."""
+    import torch
+    for longest in (40, 512, 513, 2048, 8192, 8193):
+        if batch > 4 and longest > 2048:
+            continue
+        lens = [longest, 1, 0, 16, longest - 17, 17, 255, 33]
+        seqs = [((4, 1, 2, 3, 0)[(i + longest) % 5], min(longest, lens[i % 8])) for i in range(batch)]
+        if all(n == 0 for n, _ in seqs):
+            seqs[0] = (1, seqs[0][1])
+        c = make(seqs, seed=batch, first_row=2, rows_behind=1, gate=batch % 2 == 0)
+        w = before = None
+        if weights:
+            before = torch.rand((batch, NKV, c["lmax"]), device="cuda")
+            w = before.clone()
+        got = call(cuda, c, weights=w)
+        torch.cuda.synchronize()
+        assert cuda.device_error() == (0, 0)
+        check(c, got, reference(c), w, before)
+
+
+def test_slots_in_line_form(cuda):
+    import torch
+    c = in_line_form(make([(2, 300), (1, 77), (2, 500)], seed=8))
+    before = torch.rand((6, NKV, c["lmax"]), device="cuda")
+    w, slots = before.clone(), [4, 0, 5]
+    got = call(cuda, c, weights=w, slots=torch.tensor(slots, dtype=torch.int32, device="cuda"))
+    check(c, got, reference(c), w, before, slots)
+    for bad in ([4, 4, 5], [4, -1, 5], [4, 6, 5]):
+        w2 = before.clone()
+        call(cuda, c, weights=w2, slots=torch.tensor(bad, dtype=torch.int32, device="cuda"))
+        assert cuda.device_error() == (702, 1)
+        assert torch.equal(w2[4], w[4]) and torch.equal(w2[5], w[5]) and torch.equal(w2[0], before[0])
+
+
+@pytest.mark.parametrize("seqs", [[(1 + i % 4, 100 + 237 * i) for i in range(8)], [(4, 6000)], [(2, 300)] * 37])
+def test_clusters_give_the_same_bits_over_many_launches(cuda, seqs):
+    import torch
+    c = make(seqs, seed=21, gate=True)
+    runs = []
+    ws = torch.empty(cuda.chunk_workspace_bytes(len(seqs), c["rows"], c["qmax"], c["lmax"], True), dtype=torch.uint8, device="cuda")
+    for _ in range(200):
+        w = torch.ones((len(seqs), NKV, c["lmax"]), device="cuda")
+        runs.append((*call(cuda, c, weights=w, workspace=ws), w))
+    for r in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], r))
