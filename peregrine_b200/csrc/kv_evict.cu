@@ -29,7 +29,7 @@ namespace {
 // The histogram has a column per lane: lane l adds to hist[part][l], its own bank, so a warp's adds
 // never meet however the weights cluster (attention weights share a few exponents; with one shared
 // column those adds ran one after the other: 519 us for 64 sequences of up to 65536 tokens).
-// Measured: 51 us for those 64 sequences (48 MB, 8 us at the copy rate), 8.0 us for one of 4097, 21.6 us
+// Measured: 51 us for those 64 sequences (48 MB, 8 us at the copy rate), 7.0 us for one of 4097, 21.6 us
 // for one of 262144. What bounds it are the instructions issued and the ends of the phases: a CTA takes 20
 // to 30 thousand cycles, two histograms and the list half of them, a third of that at barriers.
 constexpr int kBins = 256;
@@ -453,10 +453,11 @@ cudaError_t launch_evict_select(const float *weights, float *weights_out, int64_
     // CTAs an SM: 52.8 us against 56.4 with 1024 for 64 rows of up to 65536, 28 against 50 for 800 rows of
     // up to 8192) except above kLongRow tokens, which only 1024 hold; a batch that leaves SMs free takes
     // more CTAs, up to 8, down to kSplitPer weights a thread, below which the cluster's barriers cost more
-    // than they save. Clusters of 16 CTAs took 20 us instead of 21.6 for one sequence of 262144, but 62.7
+    // than they save (8, 12, 16 a thread, us: one sequence of 4097 8.1, 7.0, 7.0, of 16000 8.9, 8.8, 10.2, of
+    // 32000 10.0, 10.0, 10.9; 16 of 6000 10.1, 8.0, 8.2). Clusters of 16 CTAs took 20 us instead of 21.6 for one sequence of 262144, but 62.7
     // instead of 60.5 for eight and 12.9 instead of 11.3 for one of 65536. A CTA a row that reads it from
     // L2 in every round took 51 us for one sequence of 262144 and 146 us for the 64 rows.
-    constexpr int kSplitPer = 8, kLongRow = 8 * 512 * kMaxPer;
+    constexpr int kSplitPer = 12, kLongRow = 8 * 512 * kMaxPer;
     int sms = 148, dev = 0;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -486,7 +487,7 @@ cudaError_t launch_evict_select(const float *weights, float *weights_out, int64_
     const Variant &v = variants[threads == 1024 ? 3 : per <= 8 ? 0 : per <= 16 ? 1 : 2];
     // A row takes the fewest CTAs that hold it where the grid fills the device, so that the others leave
     // at once and make room; else as many as have kSplitPer weights a thread.
-    p.share = threads * ((int64_t)batch * kNumKvHeads * ctas * threads > (int64_t)sms * 1024 ? v.per : kSplitPer);
+    p.share = threads * ((int64_t)batch * kNumKvHeads * ctas * threads > (int64_t)sms * 1024 ? v.per : std::min(v.per, kSplitPer));
     const int held = std::max((per + 3) / 4 * 4, p.share / threads);  // weights a thread, at most
     const size_t smem = hist_bytes + (weights_out != nullptr ? (size_t)held * threads * sizeof(float) : 0);
     cudaLaunchConfig_t cfg = {};
