@@ -29,7 +29,7 @@ namespace {
 // The histogram has a column per lane: lane l adds to hist[part][l], its own bank, so a warp's adds
 // never meet however the weights cluster (attention weights share a few exponents; with one shared
 // column those adds ran one after the other: 519 us for 64 sequences of up to 65536 tokens).
-// Measured: 51 us for those 64 sequences (48 MB, 8 us at the copy rate), 7.0 us for one of 4097, 21.6 us
+// Measured: 43 us for those 64 sequences (48 MB, 8 us at the copy rate), 7.0 us for one of 4097, 21.6 us
 // for one of 262144. What bounds it are the instructions issued and the ends of the phases: a CTA takes 20
 // to 30 thousand cycles, two histograms and the list half of them, a third of that at barriers.
 constexpr int kBins = 256;
@@ -450,7 +450,7 @@ cudaError_t launch_evict_select(const float *weights, float *weights_out, int64_
     p.kept = kept;
     p.new_lens = new_lens;
     // Threads and CTAs per row: at least what keeps a thread within kMaxPer weights, 512 threads a CTA (two
-    // CTAs an SM: 52.8 us against 56.4 with 1024 for 64 rows of up to 65536, 28 against 50 for 800 rows of
+    // CTAs an SM: 43.0 us against 45.4 with 1024 for 64 rows of up to 65536, 28 against 50 for 800 rows of
     // up to 8192) except above kLongRow tokens, which only 1024 hold; a batch that leaves SMs free takes
     // more CTAs, up to 8, down to kSplitPer weights a thread, below which the cluster's barriers cost more
     // than they save (8, 12, 16 a thread, us: one sequence of 4097 8.1, 7.0, 7.0, of 16000 8.9, 8.8, 10.2, of
@@ -487,7 +487,8 @@ cudaError_t launch_evict_select(const float *weights, float *weights_out, int64_
     const Variant &v = variants[threads == 1024 ? 3 : per <= 8 ? 0 : per <= 16 ? 1 : 2];
     // A row takes the fewest CTAs that hold it where the grid fills the device, so that the others leave
     // at once and make room; else as many as have kSplitPer weights a thread.
-    p.share = threads * ((int64_t)batch * kNumKvHeads * ctas * threads > (int64_t)sms * 1024 ? v.per : std::min(v.per, kSplitPer));
+    const bool fills = (int64_t)batch * kNumKvHeads * ctas * threads > (int64_t)sms * 1024;
+    p.share = threads * (fills ? v.per : std::min(v.per, kSplitPer));
     const int held = std::max((per + 3) / 4 * 4, p.share / threads);  // weights a thread, at most
     const size_t smem = hist_bytes + (weights_out != nullptr ? (size_t)held * threads * sizeof(float) : 0);
     cudaLaunchConfig_t cfg = {};
@@ -495,18 +496,23 @@ cudaError_t launch_evict_select(const float *weights, float *weights_out, int64_
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
+    cudaLaunchAttribute attr[3];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = ctas;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    attr[2].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[2].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
+    // the default policy left a third of the SMs idle where CTAs leave early: 51.4 us instead of 43.0 for 64
+    // rows of up to 65536
+    attr[1].id = cudaLaunchAttributeClusterSchedulingPolicyPreference;
+    attr[1].val.clusterSchedulingPolicyPreference =
+        fills ? cudaClusterSchedulingPolicyLoadBalancing : cudaClusterSchedulingPolicyDefault;
 #ifndef PGC_NO_PDL
-    cfg.numAttrs = 2;
+    cfg.numAttrs = 3;
 #else
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
 #endif
     return cudaLaunchKernelEx(&cfg, v.kern, p);
 }
