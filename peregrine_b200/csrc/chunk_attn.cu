@@ -54,7 +54,9 @@ struct PairTiling {
     static constexpr int kTok = 64, kKeys = 128;
     static constexpr bool kWarpScan = false;
     static constexpr int kOver = 4;  // measured: 10 to 12 thousand cycles a unit, 2600 a tile
-    static constexpr int kMinShare = 8;
+    // at least one tile behind a lead: 26.2 us against 32.6 with 8 for 3 chunks of up to 90 over 1500, 23.7
+    // against 26.8 for 20 rows over 3000
+    static constexpr int kMinShare = 5;
 };
 struct SplitTiling {
     static constexpr int kTok = PGC_MAX_QUERIES, kKeys = kPage;
