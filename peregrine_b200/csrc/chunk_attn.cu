@@ -356,12 +356,6 @@ __device__ __forceinline__ void bulk_load(void *smem_dst, const void *src, uint3
                  : "memory");
 }
 
-// Hands a stage back to the producer once `data`, the last register loaded from it, has arrived: the
-// barrier's address depends on it through a value that is 0 at run time (the grid is one-dimensional).
-// Program order alone did not hold the last ldmatrix before the arrival: about once in 60 000 launches
-// it read the stage's next page in the last 16 dims.
-__device__ __forceinline__ void release_stage(uint64_t *bar, uint32_t data) { mbar_arrive(bar + (data & blockIdx.z)); }
-
 // One (page, kv head) of a pool, by its pool_page_map.
 __device__ __forceinline__ void tma_load_page(void *smem_dst, const void *tmap, int32_t row, uint64_t *bar, uint64_t policy) {
     asm volatile(
@@ -748,7 +742,7 @@ __global__ void __launch_bounds__(kCluster ? ClusterSmem::kThreads : LineSmem::k
                 mma_bf16_16816(o[2 * nd + 1], pa0, pa1, pa2, pa3, b2, b3);
             }
             __syncwarp();
-            if (lane == 0) release_stage(&empty[s], b3);
+            if (lane == 0) release_stage(&empty[s], b3, blockIdx.z);  // a one-dimensional grid: 0
         }
 
         // ------------------------------------------------------------ join the 4 warp states

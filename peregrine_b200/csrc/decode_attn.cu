@@ -63,6 +63,7 @@ struct SplitParams {
     // coherently through L2); `prefetch_ahead` pages past the ring while streaming.
     int prefetch_pre, prefetch_ahead;
     const uint8_t *k_base, *v_base;
+    uint32_t zero = 0;  // what release_stage ties a stage's hand-over to
 };
 
 struct SmemLayout {
@@ -450,15 +451,15 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
 
         // O[16 x 256] += P[16 x 16] V[16 x 256]
+        uint32_t b0, b1, b2, b3;
 #pragma unroll
         for (int nd = 0; nd < 16; ++nd) {
-            uint32_t b0, b1, b2, b3;
             ldsm_x4_trans(v_base + swz_page_offset(v_tok, nd * 16 + v_dim_off), b0, b1, b2, b3);
             mma_bf16_16816(o[2 * nd], pa0, pa1, pa2, pa3, b0, b1);
             mma_bf16_16816(o[2 * nd + 1], pa0, pa1, pa2, pa3, b2, b3);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[s]);
+        if (lane == 0) release_stage(&empty[s], b3, p.zero);
     }
 
     // ---------------------------------------------------------------- merge 4 warp states

@@ -136,6 +136,12 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// Hands a ring stage that was read by ldmatrix back to its TMA producer once `data`, the last register
+// loaded from it, has arrived: the barrier's address depends on it through `zero`, a value that is 0 at
+// run time but that the compiler cannot know. Program order alone did not hold the last ldmatrix before
+// the arrival: about once in 60 000 launches it read the stage's next page in the last 16 dims.
+__device__ __forceinline__ void release_stage(uint64_t *bar, uint32_t data, uint32_t zero) { mbar_arrive(bar + (data & zero)); }
+
 __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
