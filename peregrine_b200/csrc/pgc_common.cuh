@@ -238,6 +238,14 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
     return d;
 }
 
+// The greatest of 32 values, by four independent chains of 3-input maxima.
+__device__ __forceinline__ float max32(const float (&v)[32]) {
+    float m[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int i = 4; i < 32; i += 2) m[(i / 2) & 3] = fmax3(m[(i / 2) & 3], v[i], v[i + 1]);
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -359,13 +359,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
 #pragma unroll
                 for (int i = 0; i < 32; ++i) sv[i] = (row_ok && key0 + i <= vis) ? sv[i] : -INFINITY;
             }
-            // four independent chains of 3-input maxima
-            float mq[4] = {sv[0], sv[1], sv[2], sv[3]};
-#pragma unroll
-            for (int i = 4; i < 32; i += 8)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mq[k] = fmax3(mq[k], sv[i + 2 * k], sv[i + 2 * k + 1]);
-            float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
+            float mx = max32(sv);
             red[cg * kBM + r] = mx;
             // all four quarters have read S tile b (so P may overwrite it) and posted their max
             asm volatile("bar.sync %0, 128;" ::"r"(1 + qd) : "memory");
