@@ -271,9 +271,11 @@ size_t pgc_chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_
  * Row i of a sequence of n rows sits at position seq_lens[b] - n + i and sees the tokens up to it; a
  * row at a negative position (seq_lens[b] < n) sees nothing: out 0, lse -inf. Rows before q_starts[0]
  * and from q_starts[batch] on are left as they were. total_q, max_q_len and max_seq_len are
- * host-side bounds that size the launch: a sequence whose rows break them is skipped, one whose
- * length does counts as empty, and pgc_device_error reports either. Scores, softmax statistics and
- * sums are fp32, the probabilities are rounded to bf16 for the P.V product, the output once.
+ * host-side bounds that size the launch: a sequence of more than max_q_len rows is skipped, one whose
+ * length breaks its bound counts as empty. From the first sequence on whose q_starts descend or leave
+ * [0, total_q] all are skipped, so that no row has two owners. pgc_device_error reports each of these.
+ * Scores, softmax statistics and sums are fp32, the probabilities are rounded to bf16 for the P.V
+ * product, the output once.
  * A masked token's score is never used, whatever it is, and slots past a sequence's end are never
  * read into a sum; but a NaN or infinite V element of a cached token of the sequence makes that output
  * dim NaN in rows before the token too (its probability there is 0, and 0 times it is NaN).

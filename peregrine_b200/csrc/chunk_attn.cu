@@ -163,7 +163,9 @@ __device__ __forceinline__ void walk_start(Walk &wk, int64_t off, int64_t per, i
         if (off < c) break;
         off -= c;
     }
-    wk.left = (int)left;  // a grid of shares keeps it within int (PGC_CHUNK_MAX_ROWS)
+    // Within int from 18 shares on: the sequences' rows are disjoint, so there are at most 2^22 / 64 + 4096
+    // units a kv head, of at most 2^17 tiles and a lead.
+    wk.left = (int)left;
     walk_unit<T>(wk, (int)off);
 }
 template <class T>
@@ -176,19 +178,20 @@ __device__ __forceinline__ int64_t seq_cost(const RaggedSeq &s) {  // of one kv 
 
 // Share `index` of a grid of `grid`. Run by the whole CTA; `line` (shared memory) is written by thread
 // 0, `out` is shared memory that the larger batches go through, `cost` their scratch (one int64 per
-// sequence). Returns false when the share is empty. With kWarpScan batches of up to 128 sequences are scanned by every warp for itself,
+// sequence). Returns false when the share is empty. Sequences from the first with rows out of order on have
+// no tiles; `live` (nullable) gets the number of those before it. With kWarpScan batches of up to 128 sequences are scanned by every warp for itself,
 // which needs no barrier: 1.5 us off a single sequence's decode (in the pair kernel the registers that it
 // takes cost 2 % of the main loop).
 template <class T>
 __device__ __forceinline__ bool find_share(const RaggedBatch &rag, int64_t *cost, int index, int grid, Walk *out,
-                                           Line *line, DevError *err, Walk &wk) {
+                                           Line *line, DevError *err, Walk &wk, int *live_out = nullptr) {
     constexpr int kChunks = 4;
     const int lane = threadIdx.x & 31;
     wk.seq = -1;
     if (T::kWarpScan && rag.batch <= 32 * kChunks) {
         // a sequence has at most 2^22 tiles and leads (PGC_CHUNK_MAX_TOKENS): 32 bits hold the line
         RaggedSeq s[kChunks];
-        int c[kChunks], incl[kChunks], total = 0;
+        int c[kChunks], incl[kChunks], total = 0, live = rag.batch;
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) {
             s[k] = RaggedSeq{0, 0, 0};
@@ -198,7 +201,9 @@ __device__ __forceinline__ bool find_share(const RaggedBatch &rag, int64_t *cost
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) {
             if (k * 32 >= rag.batch) break;
-            c[k] = (int)seq_cost<T>(s[k]) * kNumKvHeads;
+            const uint32_t bad = __ballot_sync(0xffffffffu, s[k].row0 < 0);
+            if (bad != 0) live = min(live, k * 32 + __ffs(bad) - 1);
+            c[k] = k * 32 + lane < live ? (int)seq_cost<T>(s[k]) * kNumKvHeads : 0;
             incl[k] = c[k];
 #pragma unroll 1
             for (int o = 1; o < 32; o <<= 1) {
@@ -209,7 +214,10 @@ __device__ __forceinline__ bool find_share(const RaggedBatch &rag, int64_t *cost
             total = __shfl_sync(0xffffffffu, incl[k], 31);
         }
         const Line ln = make_line<T>(total, grid);
-        if (threadIdx.x == 0) *line = ln;
+        if (threadIdx.x == 0) {
+            *line = ln;
+            if (live_out != nullptr) *live_out = live;
+        }
         const int begin = (int)share_begin(ln, index), end = (int)share_begin(ln, index + 1);
         if (index >= ln.shares || end <= begin) return false;
 #pragma unroll
@@ -228,19 +236,20 @@ __device__ __forceinline__ bool find_share(const RaggedBatch &rag, int64_t *cost
         }
         return true;
     }
-    for (int b = threadIdx.x; b < rag.batch; b += blockDim.x) cost[b] = seq_cost<T>(ragged_seq(rag, b, err)) * kNumKvHeads;
+    for (int b = threadIdx.x; b < rag.batch; b += blockDim.x) {
+        const RaggedSeq s = ragged_seq(rag, b, err);
+        cost[b] = s.row0 < 0 ? -1 : seq_cost<T>(s) * kNumKvHeads;
+    }
     __syncthreads();
     if (threadIdx.x < 32) {
-        int64_t total = 0;
-        for (int b = lane; b < rag.batch; b += 32) total += cost[b];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        int live;
+        const int64_t total = ragged_total(cost, rag.batch, live);
         const Line ln = make_line<T>(total, grid);
         const int64_t begin = share_begin(ln, index), end = share_begin(ln, index + 1);
         if (index < ln.shares && end > begin) {
             int64_t before = 0;
-            for (int b0 = 0; b0 < rag.batch; b0 += 32) {
-                const int64_t c = b0 + lane < rag.batch ? cost[b0 + lane] : 0;
+            for (int b0 = 0; b0 < live; b0 += 32) {
+                const int64_t c = b0 + lane < live ? cost[b0 + lane] : 0;
                 int64_t incl = c;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -262,6 +271,7 @@ __device__ __forceinline__ bool find_share(const RaggedBatch &rag, int64_t *cost
         if (lane == 0) {
             *out = wk;
             *line = ln;
+            if (live_out != nullptr) *live_out = live;
         }
     }
     __syncthreads();
@@ -314,6 +324,7 @@ struct SplitParams {
     uint16_t *out;
     float *lse;        // nullable
     Fragment *frags;   // [batch][4]
+    int *live;         // sequences that have one: those before the first with rows out of order
     float *parts;      // [shares][2][4 * max_q_len][258]
     float *scores;     // nullable: [total_q][4][score_stride][4], scaled by log2(e)
     int64_t score_stride;
@@ -526,7 +537,9 @@ __global__ void __launch_bounds__(kCluster ? ClusterSmem::kThreads : LineSmem::k
         w.kvh = unit % kNumKvHeads;
         w.qt = 0;
         const RaggedSeq s = ragged_seq(p.rag, w.seq, unit % kNumKvHeads + rank + threadIdx.x == 0 ? &g_chunk_err : nullptr);
-        if (s.n == 0) return;  // the whole cluster
+        bool bad = s.n == 0;
+        for (int b = lane; b < w.seq; b += 32) bad |= p.rag.q_starts[b] < 0 || p.rag.q_starts[b + 1] < p.rag.q_starts[b];
+        if (__any_sync(0xffffffffu, bad)) return;  // the whole cluster
         w.row0 = s.row0;
         w.n = s.n;
         w.len = s.len;
@@ -537,7 +550,7 @@ __global__ void __launch_bounds__(kCluster ? ClusterSmem::kThreads : LineSmem::k
     } else {
         const bool busy = find_share<SplitTiling>(p.rag, reinterpret_cast<int64_t *>(smem + SplitSmem::kRing), index,
                                                   gridDim.x, reinterpret_cast<Walk *>(smem + SplitSmem::kWalk), line,
-                                                  index == 0 ? &g_chunk_err : nullptr, w);
+                                                  index == 0 ? &g_chunk_err : nullptr, w, index == 0 ? p.live : nullptr);
         if (!busy) return;
         fence_proxy_async_smem();  // the schedule's scratch becomes the ring
     }
@@ -1393,6 +1406,7 @@ struct FinishParams {
     uint16_t *out;
     float *lse;
     RaggedBatch rag;  // the split form's: its records are by (sequence, kv head)
+    const int *live;
     const float *scores;
     int64_t score_stride;
     ChunkWeights w;
@@ -1579,7 +1593,7 @@ __device__ __forceinline__ void add_weights(const FinishParams &p, int blk) {
     const Fragment f = read_record(p, unit);  // of a sequence with rows only
     const RaggedSeq sv = ragged_seq(p.rag, b, nullptr);
     const int t0 = chunk * kAddTokens;
-    if (sv.n == 0 || t0 >= sv.len) return;
+    if (b >= *p.live || sv.n == 0 || t0 >= sv.len) return;
     const int64_t slot = ragged_slot(p.w.slots, p.w.num_slots, b, chunk == 0 && kvh == 0 ? &g_chunk_err : nullptr);
     if (slot < 0) return;
     float *w = p.w.weights + (slot * kNumKvHeads + kvh) * p.w.stride;
@@ -1655,10 +1669,10 @@ __global__ void __launch_bounds__(kFinishThreads) chunk_finish_kernel(const Fini
         add_weights(p, blockIdx.x - p.merge_blocks);
         return;
     }
-    const int y = blockIdx.x % p.rows, lanes = p.merge_blocks / p.rows;
+    const int y = blockIdx.x % p.rows, lanes = p.merge_blocks / p.rows, live = *p.live;
     for (int i = blockIdx.x / p.rows; i < p.records; i += lanes) {
         const Fragment f = read_record(p, i);
-        if (ragged_seq(p.rag, i / kNumKvHeads, nullptr).n == 0 || f.first >= f.last) continue;  // uniform
+        if (i / kNumKvHeads >= live || ragged_seq(p.rag, i / kNumKvHeads, nullptr).n == 0 || f.first >= f.last) continue;  // uniform
         merge_row(p, f, y);
         __syncthreads();  // before the next record's sums
     }
@@ -1716,7 +1730,7 @@ inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 struct Layout {
     bool split;
     int shares, rows, records;  // rows: of a partial
-    size_t frags = 0, parts = 0, lse = 0, scores = 0, total = 0;
+    size_t frags = 0, live = 0, parts = 0, lse = 0, scores = 0, total = 0;
     int64_t score_stride = 0;
 };
 Layout layout(int batch, int total_q, int max_q_len, int max_seq_len, bool weights, int sm_count) {
@@ -1726,7 +1740,8 @@ Layout layout(int batch, int total_q, int max_q_len, int max_seq_len, bool weigh
     l.rows = l.split ? max_q_len * kGroup : 2 * kBM;
     const size_t part = l.split ? (size_t)l.rows * kPartial : kPairPart;
     l.records = l.split ? batch * kNumKvHeads : l.shares;
-    l.parts = align256((size_t)l.records * sizeof(Fragment));
+    l.live = (size_t)l.records * sizeof(Fragment);
+    l.parts = align256(l.live + sizeof(int));
     l.lse = align256(l.parts + (size_t)l.shares * 2 * part * sizeof(float));
     l.scores = align256(l.lse + (weights ? (size_t)total_q * kNumQHeads * sizeof(float) : 0));
     l.score_stride = (max_seq_len + kPage - 1) / kPage * kPage;
@@ -1782,6 +1797,7 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
         sp.out = out;
         sp.lse = lse;
         sp.frags = reinterpret_cast<Fragment *>(ws + lay.frags);
+        sp.live = reinterpret_cast<int *>(ws + lay.live);
         sp.parts = reinterpret_cast<float *>(ws + lay.parts);
         sp.scores = weights != nullptr ? reinterpret_cast<float *>(ws + lay.scores) : nullptr;
         sp.score_stride = lay.score_stride;
@@ -1797,6 +1813,7 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
                                            : launch_pdl(chunk_split_kernel<false, false>, grid, block, LineSmem::kAlloc, stream, tk, tv, sp);
         if (e != cudaSuccess) return e;
         fp.rag = rag;
+        fp.live = sp.live;
         // a few hundred blocks cover the records: most of a large batch's are of units not cut
         fp.merge_blocks = (lay.records < lay.shares ? lay.records : lay.shares) * lay.rows;
         int blocks = fp.merge_blocks;

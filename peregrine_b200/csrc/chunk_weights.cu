@@ -108,22 +108,20 @@ __device__ __forceinline__ bool units_next(const RaggedBatch &rag, Units &u) {
 __device__ __forceinline__ bool find_units(const RaggedBatch &rag, int64_t *cost, int pair, int pairs, Units *out) {
     for (int b = threadIdx.x; b < rag.batch; b += blockDim.x) {
         const RaggedSeq s = ragged_seq(rag, b, nullptr);
-        cost[b] = head_cost(s.n, s.len) * kNumKvHeads;
+        cost[b] = s.row0 < 0 ? -1 : head_cost(s.n, s.len) * kNumKvHeads;
     }
     __syncthreads();
     if (threadIdx.x < 32) {
         const int lane = threadIdx.x;
-        int64_t total = 0;
-        for (int b = lane; b < rag.batch; b += 32) total += cost[b];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        int live;
+        const int64_t total = ragged_total(cost, rag.batch, live);
         const int64_t begin = total * pair / pairs, end = total * (pair + 1) / pairs;
         Units u = {};
         u.seq = -1;
         if (end > begin) {
             int64_t before = 0;
-            for (int b0 = 0; b0 < rag.batch; b0 += 32) {
-                const int64_t c = b0 + lane < rag.batch ? cost[b0 + lane] : 0;
+            for (int b0 = 0; b0 < live; b0 += 32) {
+                const int64_t c = b0 + lane < live ? cost[b0 + lane] : 0;
                 int64_t incl = c;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {

@@ -8,23 +8,27 @@
 namespace pgc {
 
 struct RaggedSeq {
-    int row0;  // first query row
+    int row0;  // first query row; -1: q_starts is out of order here
     int n;     // query rows; 0: nothing to do
     int len;   // cached tokens, the queries included
 };
 
-// Sequence b. Query rows outside [0, total_q], out of order or more than max_q_len: the sequence is
-// skipped (n = 0). A length outside [0, max_seq_len]: its cache counts as empty, so its rows see
-// nothing. Both are recorded in *err (nullable: one thread of a launch records).
+// Sequence b. Query rows outside [0, total_q] or out of order: the sequence is skipped (n = 0), and so
+// are all behind it, for which the caller looks out (row0 = -1): no row then belongs to two sequences,
+// and a batch has at most total_q rows. More rows than max_q_len: the sequence is skipped. A length outside
+// [0, max_seq_len]: its cache counts as empty, so its rows see nothing. All are recorded in *err
+// (nullable: one thread of a launch records).
 __device__ __forceinline__ RaggedSeq ragged_seq(const RaggedBatch &r, int b, DevError *err) {
     RaggedSeq s;
     const int end = r.q_starts[b + 1];
     s.row0 = r.q_starts[b];
     s.len = r.seq_lens[b];
     // 0 <= row0 <= end <= total_q is checked first, so the difference cannot overflow
-    if (s.row0 < 0 || end < s.row0 || end > r.total_q || end - s.row0 > r.max_q_len) {
+    const bool in_order = s.row0 >= 0 && end >= s.row0 && end <= r.total_q;
+    if (!in_order || end - s.row0 > r.max_q_len) {
         if (err != nullptr) record_error(err, kErrRowsOutOfRange, b);
-        s.row0 = s.n = 0;
+        s.row0 = in_order ? 0 : -1;
+        s.n = 0;
         return s;
     }
     s.n = end - s.row0;
@@ -33,6 +37,29 @@ __device__ __forceinline__ RaggedSeq ragged_seq(const RaggedBatch &r, int b, Dev
         s.len = 0;
     }
     return s;
+}
+
+// The sum of the costs of the sequences before the first whose cost is -1 (rows out of order), and their
+// number. Called by a whole warp.
+__device__ __forceinline__ int64_t ragged_total(const int64_t *cost, int batch, int &live) {
+    const int lane = threadIdx.x & 31;
+    auto sum = [&](int end, int &first_bad) {
+        int64_t total = 0;
+        for (int b = lane; b < end; b += 32) {
+            if (cost[b] < 0)
+                first_bad = min(first_bad, b);
+            else
+                total += cost[b];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        first_bad = __reduce_min_sync(0xffffffffu, first_bad);
+        return total;
+    };
+    live = batch;
+    int64_t total = sum(batch, live);
+    if (live < batch) total = sum(live, live);
+    return total;
 }
 
 // Slot of sequence b in a slot-indexed array, -1 when it may not be used: outside [0, num_slots),
