@@ -44,6 +44,13 @@ __device__ __forceinline__ float sigmoid_gate(float v, uint32_t gate_bits) {
     return v * r;
 }
 
+// A row's log-sum-exp as the weights take it: in log2 units, in which the scores are, since the way through
+// natural units and back rounds three times where |m| is large; +inf for a row whose sum is 0, so that
+// its -inf scores add nothing. Partials hold their maxima in log2 units too.
+__device__ __forceinline__ float lse_log2(float m, float sum) { return sum == 0.f ? INFINITY : m + log2f(sum); }
+// The same for the caller: natural units, -inf for such a row.
+__device__ __forceinline__ float lse_natural(float m, float sum) { return sum == 0.f ? -INFINITY : m * kLn2 + logf(sum); }
+
 // =============================================================================================
 // The schedule. A unit is a (sequence, kv head, block of kTok query tokens); its tiles are blocks of
 // kKeys keys. The line of work is the units' tiles, units in that order, each unit preceded by the
@@ -323,6 +330,7 @@ struct SplitParams {
     const uint16_t *gate;
     uint16_t *out;
     float *lse;        // nullable
+    float *lse2;       // nullable: as the weights take it (lse_log2)
     Fragment *frags;   // [batch][4]
     int *live;         // sequences that have one: those before the first with rows out of order
     float *parts;      // [shares][2][4 * max_q_len][258]
@@ -466,9 +474,8 @@ __device__ __forceinline__ void join_cluster(const SplitParams &p, uint8_t *ring
         }
         *reinterpret_cast<uint32_t *>(p.out + out_row(r) * kHeadDim + d) = pack_bf16x2(acc.x, acc.y);
         if (e % pairs == 0) {
-            // +inf for a row whose sum is 0, so that its -inf scores add nothing
-            if (kScores) lse2[r] = den == 0.f ? INFINITY : mx + log2f(den);
-            if (rank == 0 && p.lse != nullptr) p.lse[out_row(r)] = den == 0.f ? -INFINITY : mx * kLn2 + logf(den);
+            if (kScores) lse2[r] = lse_log2(mx, den);
+            if (rank == 0 && p.lse != nullptr) p.lse[out_row(r)] = lse_natural(mx, den);
         }
     }
     if (kScores) {
@@ -800,7 +807,7 @@ __global__ void __launch_bounds__(kCluster ? ClusterSmem::kThreads : LineSmem::k
             if (!whole) {
                 float *dst = part + r * kPartial;
                 *reinterpret_cast<float2 *>(dst + 2 + d) = acc;
-                if (d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(ma * kLn2, den);
+                if (d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(ma, den);
                 return;
             }
             const int64_t row = out_row(r);
@@ -812,7 +819,8 @@ __global__ void __launch_bounds__(kCluster ? ClusterSmem::kThreads : LineSmem::k
                 acc.y = sigmoid_gate(acc.y, gv >> 16);
             }
             *reinterpret_cast<uint32_t *>(p.out + row * kHeadDim + d) = pack_bf16x2(acc.x, acc.y);
-            if (d == 0 && p.lse != nullptr) p.lse[row] = den == 0.f ? -INFINITY : ma * kLn2 + logf(den);
+            if (d == 0 && p.lse != nullptr) p.lse[row] = lse_natural(ma, den);
+            if (kScores && d == 0) p.lse2[row] = lse_log2(ma, den);
         };
         // the share's last unit: the ring and Q are free, and hold all rows at once
         const bool last = walk_last<SplitTiling>(w);
@@ -918,6 +926,7 @@ struct PairParams {
     const uint16_t *gate;
     uint16_t *out;
     float *lse;
+    float *lse2;      // nullable
     Fragment *frags;  // [pairs]
     float *parts;     // [pairs][2][kPairPart]
     float scale_log2;
@@ -1326,10 +1335,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 float *part = p.parts + (int64_t)(pair * 2 + slot) * kPairPart + rank * kBM + r;
                 if (cg == 0) {
                     if (!whole) {
-                        part[kPairStat] = (m == -INFINITY) ? -INFINITY : m * kLn2;
+                        part[kPairStat] = m;
                         part[kPairStat + 2 * kBM] = l_row;
-                    } else if (row_ok && p.lse != nullptr) {
-                        p.lse[orow] = l_row == 0.f ? -INFINITY : m * kLn2 + logf(l_row);
+                    } else if (row_ok) {
+                        if (p.lse != nullptr) p.lse[orow] = lse_natural(m, l_row);
+                        if (p.lse2 != nullptr) p.lse2[orow] = lse_log2(m, l_row);
                     }
                 }
 #pragma unroll
@@ -1405,6 +1415,7 @@ struct FinishParams {
     const uint16_t *gate;
     uint16_t *out;
     float *lse;
+    float *lse2;  // nullable; written behind the pair kernel, read behind the split kernel
     RaggedBatch rag;  // the split form's: its records are by (sequence, kv head)
     const int *live;
     const float *scores;
@@ -1461,14 +1472,14 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const Finish
 #pragma unroll
         for (int j = 0; j < kFrags; ++j) mx = fmaxf(mx, m[j]);
         const float base_m = mx == -INFINITY ? 0.f : mx;  // nothing seen so far: all weights 0
-        const float corr = fast_exp2((ma - base_m) * kLog2e);
+        const float corr = fast_exp2(ma - base_m);
         ma = mx;
         den *= corr;
 #pragma unroll
         for (int k = 0; k < 2; ++k) acc[k] = make_float4(acc[k].x * corr, acc[k].y * corr, acc[k].z * corr, acc[k].w * corr);
 #pragma unroll
         for (int j = 0; j < kFrags; ++j) {
-            const float w = fast_exp2((m[j] - base_m) * kLog2e);
+            const float w = fast_exp2(m[j] - base_m);
             den += l[j] * w;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -1488,8 +1499,11 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const Finish
         to[2] = acc[k].z * inv;
         to[3] = acc[k].w * inv;
     }
-    if (warp == 0 && blockIdx.z == 0 && p.lse != nullptr && r < nrows)
-        p.lse[(int64_t)(f.row + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup] = (den == 0.f) ? -INFINITY : ma + logf(den);
+    if (warp == 0 && blockIdx.z == 0 && r < nrows) {
+        const int64_t orow = (int64_t)(f.row + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup;
+        if (p.lse != nullptr) p.lse[orow] = lse_natural(ma, den);
+        if (p.lse2 != nullptr) p.lse2[orow] = lse_log2(ma, den);
+    }
     __syncthreads();
     // 8 threads a row, 8 dims each
     const int rr = threadIdx.x >> 3, row = blockIdx.y * 32 + rr, d = (threadIdx.x & 7) * 8;
@@ -1545,14 +1559,14 @@ __device__ __forceinline__ void merge_row(const FinishParams &p, const Fragment 
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) mx = fmaxf(mx, ml[j].x);
         const float base_m = mx == -INFINITY ? 0.f : mx;
-        const float corr = fast_exp2((ma - base_m) * kLog2e);
+        const float corr = fast_exp2(ma - base_m);
         ma = mx;
         den *= corr;
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[k] = __fmul2_rn(acc[k], make_float2(corr, corr));
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            const float w = fast_exp2((ml[j].x - base_m) * kLog2e);
+            const float w = fast_exp2(ml[j].x - base_m);
             den += ml[j].x == -INFINITY ? 0.f : ml[j].y * w;
 #pragma unroll
             for (int k = 0; k < 4; ++k) acc[k] = __ffma2_rn(v[j][k], make_float2(w, w), acc[k]);
@@ -1571,7 +1585,7 @@ __device__ __forceinline__ void merge_row(const FinishParams &p, const Fragment 
     float mx = mine.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float scale = mine.x == -INFINITY ? 0.f : fast_exp2((mine.x - mx) * kLog2e);
+    const float scale = mine.x == -INFINITY ? 0.f : fast_exp2(mine.x - mx);
     den = mine.y * scale;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
@@ -1580,7 +1594,7 @@ __device__ __forceinline__ void merge_row(const FinishParams &p, const Fragment 
     for (int w = 0; w < kFinishWarps; ++w) sum += red[w][d] * __shfl_sync(0xffffffffu, scale, w);
     const float o = den == 0.f ? 0.f : sum / den * gate;
     p.out[orow * kHeadDim + d] = f32_to_bf16_bits(o);
-    if (p.lse != nullptr && d == 0) p.lse[orow] = (den == 0.f) ? -INFINITY : mx + logf(den);
+    if (p.lse != nullptr && d == 0) p.lse[orow] = lse_natural(mx, den);
 }
 
 // The weights of 2048 tokens of one (sequence, kv head) from the scores that the split kernel left and
@@ -1616,7 +1630,7 @@ __device__ __forceinline__ void add_weights(const FinishParams &p, int blk) {
     }
     load_scores(0);
     {
-        // 16 threads a row (the first half of the block); +inf for a row whose sum is 0, so that its -inf scores add nothing
+        // 16 threads a row (the first half of the block)
         const int r = threadIdx.x >> 4, lane16 = threadIdx.x & 15;
         const bool mine = r < sv.n * kGroup;  // sv.n <= 4
         float m = -INFINITY, l = 0.f;
@@ -1627,22 +1641,18 @@ __device__ __forceinline__ void add_weights(const FinishParams &p, int blk) {
                 const float2 ml = *reinterpret_cast<const float2 *>(base + fragment_at(p, i));
                 const float mx = fmaxf(m, ml.x);
                 if (mx == -INFINITY) continue;
-                l = l * exp2f((m - mx) * kLog2e) + ml.y * exp2f((ml.x - mx) * kLog2e);
+                l = l * exp2f(m - mx) + ml.y * exp2f(ml.x - mx);
                 m = mx;
             }
             float mx = m;
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            l = m == -INFINITY ? 0.f : l * exp2f((m - mx) * kLog2e);
+            l = m == -INFINITY ? 0.f : l * exp2f(m - mx);
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (lane16 == 0 && r < kRows) lse2[r] = l == 0.f ? INFINITY : mx * kLog2e + log2f(l);
+            if (lane16 == 0 && r < kRows) lse2[r] = lse_log2(mx, l);
         } else if (lane16 == 0 && r < kRows) {
-            lse2[r] = INFINITY;
-            if (mine) {
-                const float v = p.lse[(int64_t)(sv.row0 + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup];
-                if (v != -INFINITY) lse2[r] = v * kLog2e;
-            }
+            lse2[r] = mine ? p.lse2[(int64_t)(sv.row0 + r / kGroup) * kNumQHeads + kvh * kGroup + r % kGroup] : INFINITY;
         }
     }
     __syncthreads();
@@ -1777,7 +1787,7 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
     }
     const Layout lay = layout(rag.batch, rag.total_q, rag.max_q_len, rag.max_seq_len, weights != nullptr, sm_count);
     uint8_t *ws = static_cast<uint8_t *>(workspace);
-    if (lse == nullptr && weights != nullptr) lse = reinterpret_cast<float *>(ws + lay.lse);
+    float *lse2 = weights != nullptr ? reinterpret_cast<float *>(ws + lay.lse) : nullptr;
     FinishParams fp = {};
     fp.frags = reinterpret_cast<const Fragment *>(ws + lay.frags);
     fp.parts = reinterpret_cast<const float *>(ws + lay.parts);
@@ -1786,6 +1796,7 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
     fp.gate = gate;
     fp.out = out;
     fp.lse = lse;
+    fp.lse2 = lse2;
     if (lay.split) {
         SplitParams sp = {};
         sp.rag = rag;
@@ -1796,6 +1807,7 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
         sp.gate = gate;
         sp.out = out;
         sp.lse = lse;
+        sp.lse2 = lse2;
         sp.frags = reinterpret_cast<Fragment *>(ws + lay.frags);
         sp.live = reinterpret_cast<int *>(ws + lay.live);
         sp.parts = reinterpret_cast<float *>(ws + lay.parts);
@@ -1837,13 +1849,14 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
     pp.gate = gate;
     pp.out = out;
     pp.lse = lse;
+    pp.lse2 = lse2;
     pp.frags = reinterpret_cast<Fragment *>(ws + lay.frags);
     pp.parts = reinterpret_cast<float *>(ws + lay.parts);
     pp.scale_log2 = scale * kLog2e;
     cudaError_t e = launch_pdl(chunk_pair_kernel, dim3(2 * lay.shares), dim3(kPairThreads), PairSmem::kBytes, stream, tq, tk, tv, pp);
     if (e == cudaSuccess) e = launch_pdl(chunk_merge_kernel, dim3(lay.shares, lay.rows / 32, kHeadDim / kMergeDims), dim3(kMergeThreads), 0, stream, fp);
     if (e != cudaSuccess || weights == nullptr) return e;
-    return launch_chunk_weights(q, tk, num_pages, block_tables, max_pages_per_seq, rag, scale, lse, *weights, sm_count, stream);
+    return launch_chunk_weights(q, tk, num_pages, block_tables, max_pages_per_seq, rag, scale, lse2, *weights, sm_count, stream);
 }
 
 cudaError_t chunk_read_error(DevErrorHost *e, bool clear) {

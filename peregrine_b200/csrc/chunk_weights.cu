@@ -46,7 +46,7 @@ struct WeightsParams {
     const int32_t *block_tables;
     int max_pages_per_seq;
     int64_t num_pages;
-    const float *lse;
+    const float *lse2;  // of the attention's rows, in log2 units; +inf for a row that sees nothing
     ChunkWeights w;
     float scale_log2;
 };
@@ -349,13 +349,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float *sum_s = reinterpret_cast<float *>(smem + Smem::kSum);
         const uint32_t ebar = leader_addr(&d_empty[grp]);
         const float c = p.scale_log2;
-        // Column gtid's lse in log2 units; +inf for a row whose sum is 0, so that its -inf scores add
-        // nothing, and for the rows that are not the sequence's.
+        // Column gtid's lse in log2 units; +inf, with which it adds nothing, for the rows that are not the
+        // sequence's too.
         auto load_lse = [&](int qt) -> float {
             const int tok = qt * kTileTok + gtid / kGroup;
             if (tok >= u.n) return INFINITY;
-            const float x = p.lse[(int64_t)(u.row0 + tok) * kNumQHeads + u.kvh * kGroup + gtid % kGroup];
-            return x == -INFINITY ? INFINITY : x * kLog2e;
+            return p.lse2[(int64_t)(u.row0 + tok) * kNumQHeads + u.kvh * kGroup + gtid % kGroup];
         };
         int tile = 0, slot_seq = -1;  // tile: the share's tiles before this unit
         int64_t slot = -1;
@@ -446,7 +445,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 cudaError_t launch_chunk_weights(const uint16_t *q, const CUtensorMap &tk, int64_t num_pages,
                                  const int32_t *block_tables, int max_pages_per_seq, const RaggedBatch &rag,
-                                 float scale, const float *lse, const ChunkWeights &weights, int sm_count,
+                                 float scale, const float *lse2, const ChunkWeights &weights, int sm_count,
                                  cudaStream_t stream) {
     static std::atomic<bool> attr_set[64] = {};
     int dev = 0;
@@ -464,7 +463,7 @@ cudaError_t launch_chunk_weights(const uint16_t *q, const CUtensorMap &tk, int64
     wp.block_tables = block_tables;
     wp.max_pages_per_seq = max_pages_per_seq;
     wp.num_pages = num_pages;
-    wp.lse = lse;
+    wp.lse2 = lse2;
     wp.w = weights;
     wp.scale_log2 = scale * kLog2e;
     return launch_pdl(chunk_weights_kernel, dim3(sm_count / 2 * 2), dim3(kThreads), Smem::kBytes, stream, tq, tk, wp);

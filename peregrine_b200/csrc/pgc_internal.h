@@ -142,10 +142,11 @@ cudaError_t launch_chunk(const uint16_t *q, const CUtensorMap &tk, const CUtenso
                          const ChunkWeights *weights, void *workspace, int sm_count, cudaStream_t stream);
 cudaError_t chunk_read_error(DevErrorHost *e, bool clear);
 
-// chunk_weights.cu: weights += column sums of exp(scale q.k - lse) over the batch's rows
+// chunk_weights.cu: weights += column sums of exp(scale q.k - lse) over the batch's rows; lse2 is the
+// rows' lse in log2 units, +inf for a row that sees nothing
 cudaError_t launch_chunk_weights(const uint16_t *q, const CUtensorMap &tk, int64_t num_pages,
                                  const int32_t *block_tables, int max_pages_per_seq, const RaggedBatch &rag,
-                                 float scale, const float *lse, const ChunkWeights &weights, int sm_count,
+                                 float scale, const float *lse2, const ChunkWeights &weights, int sm_count,
                                  cudaStream_t stream);
 cudaError_t chunk_weights_read_error(DevErrorHost *e, bool clear);
 
