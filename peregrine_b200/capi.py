@@ -10,6 +10,7 @@ device-memory allocator and stream source) and raise PgcError on a non-zero stat
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libperegrine_cuda.so"
@@ -242,11 +243,22 @@ def _ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+@functools.cache
+def _torch_current():
+    """Functions for torch's current device and for the raw handle of a device's current stream: torch's
+    inner ones (0.1 us each), or, in a torch that has them no more, the public ones (3 us for the
+    torch.cuda.Stream object)."""
+    import torch
+    device, raw = (getattr(torch._C, name, None) for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
+    if device is None or raw is None:
+        return torch.cuda.current_device, lambda d: torch.cuda.current_stream(d).cuda_stream
+    return device, raw
+
+
 def _stream(stream) -> int | None:
     if stream is None:
-        import torch
-        # the raw handle: a torch.cuda.Stream object for it costs 3 us a call
-        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+        device, raw = _torch_current()
+        return raw(device())
     return getattr(stream, "cuda_stream", stream)
 
 
