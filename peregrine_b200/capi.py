@@ -40,6 +40,7 @@ STATUS = {
 
 
 STATUS_INVALID = -1
+STATUS_BOUNDS = -2
 
 
 class PgcError(RuntimeError):
@@ -262,6 +263,40 @@ def _stream(stream) -> int | None:
     return getattr(stream, "cuda_stream", stream)
 
 
+@functools.cache
+def _dtypes():
+    """The types of bf16 arrays (or their bits), of indices and of fp32 arrays."""
+    import torch
+    return (torch.bfloat16, torch.int16, torch.uint16), (torch.int32,), (torch.float32,)
+
+
+def _refuse(what: str, *tensors) -> None:
+    """Raises for the first of `tensors` that the kernels could not use as they do, an access out of range on
+    the GPU for the most part. Each is (name, tensor or None, dtypes, bytes, whether exactly, not at least);
+    all are to be contiguous and on the current device. The entries below first ask for as much in one
+    expression, of as few attributes as that takes, at some 60 ns each in calls of 6 to 12 us: an index array
+    of exactly 4 bytes an element needs no look at its type."""
+    for name, t, dtypes, nbytes, exact in tensors:
+        if t is None:
+            continue
+        if t.dtype not in dtypes or not t.is_contiguous():
+            raise PgcError(STATUS_INVALID, f"{what}: {name} is {t.dtype}, contiguous: {t.is_contiguous()}")
+        if t.nbytes != nbytes if exact else t.nbytes < nbytes:
+            raise PgcError(STATUS_BOUNDS, f"{what}: {name} has {t.nbytes} bytes, not {nbytes}")
+    current = _torch_current()[0]()
+    for name, t, *_ in tensors:
+        if t is not None and t.get_device() != current:
+            raise PgcError(STATUS_INVALID, f"{what}: {name} is on {t.device}, not the current CUDA device")
+
+
+def _dims(what: str, name: str, t, *dims):
+    """t's shape, of which the given dims (None: any) are fixed."""
+    shape = t.shape
+    if len(shape) != len(dims) or any(d is not None and d != s for d, s in zip(dims, shape)):
+        raise PgcError(STATUS_BOUNDS, f"{what}: {name} has the shape {tuple(shape)}")
+    return shape
+
+
 def decode_workspace_bytes(batch: int, num_queries: int, max_seq_len: int) -> int:
     return int(lib().pgc_decode_workspace_bytes(batch, num_queries, max_seq_len))
 
@@ -345,43 +380,133 @@ def chunk_workspace_bytes(batch: int, total_q: int, max_q_len: int, max_seq_len:
     return int(lib().pgc_chunk_workspace_bytes(batch, total_q, max_q_len, max_seq_len, int(with_weights)))
 
 
+_Q_ROW = NUM_Q_HEADS * HEAD_DIM * 2                  # bytes of a query row
+_POOL_PAGE = NUM_KV_HEADS * PAGE_TOKENS * HEAD_DIM * 2  # and of a pool's page
+
+
+def _chunk_shape(what, device, q, k_pages, v_pages, block_tables, q_starts, seq_lens, out, workspace, gate, lse):
+    """(query rows, pages, table width, batch) of a ragged batch whose tensors agree."""
+    b16, i32, f32 = _dtypes()
+    rows, pages, batch = q.shape[0], k_pages.shape[0], seq_lens.shape[0]
+    tables, width = block_tables.shape if block_tables.ndim == 2 else (-1, 0)
+    q_bytes, pool_bytes = rows * _Q_ROW, pages * _POOL_PAGE
+    if (tables >= batch and q.nbytes == q_bytes and out.nbytes >= q_bytes and k_pages.nbytes == v_pages.nbytes == pool_bytes
+            and block_tables.nbytes == 4 * tables * width and q_starts.nbytes == 4 * batch + 4 and seq_lens.nbytes == 4 * batch
+            and q.dtype in b16 and out.dtype in b16 and k_pages.dtype in b16
+            and q.is_contiguous() and out.is_contiguous() and k_pages.is_contiguous() and v_pages.is_contiguous()
+            and block_tables.is_contiguous() and q_starts.is_contiguous() and seq_lens.is_contiguous()
+            and workspace.is_contiguous()
+            and device == q.get_device() == out.get_device() == k_pages.get_device() == v_pages.get_device()
+            == block_tables.get_device() == q_starts.get_device() == seq_lens.get_device() == workspace.get_device()
+            and (gate is None or (gate.nbytes >= q_bytes and gate.dtype in b16 and gate.is_contiguous() and gate.get_device() == device))
+            and (lse is None or (lse.nbytes >= rows * NUM_Q_HEADS * 4 and lse.dtype in f32 and lse.is_contiguous()
+                                 and lse.get_device() == device))):
+        return rows, pages, width, batch
+    _dims(what, "seq_lens", seq_lens, None)
+    tables, width = _dims(what, "block_tables", block_tables, None, None)
+    _refuse(what, ("q", q, b16, q_bytes, True), ("k_pages", k_pages, b16, pool_bytes, True),
+            ("v_pages", v_pages, b16, pool_bytes, True), ("block_tables", block_tables, i32, 4 * batch * width, False),
+            ("q_starts", q_starts, i32, 4 * batch + 4, True), ("seq_lens", seq_lens, i32, 4 * batch, True),
+            ("out", out, b16, q_bytes, False), ("gate", gate, b16, q_bytes, False),
+            ("lse", lse, f32, rows * NUM_Q_HEADS * 4, False), ("workspace", workspace, (workspace.dtype,), 0, False))
+    return rows, pages, width, batch
+
+
 def chunk_attn(q, k_pages, v_pages, block_tables, q_starts, seq_lens, max_q_len, max_seq_len, scale, out,
                workspace, gate=None, lse=None, stream=None) -> None:
     """pgc_chunk_attn: causal attention of a ragged batch; q/out [total_q][16][256], q_starts
-    [batch + 1] and seq_lens [batch] int32 on the device, lse fp32 [total_q][16]."""
+    [batch + 1] and seq_lens [batch] int32 on the device, lse fp32 [total_q][16]. All contiguous and on the
+    current device; out, gate and lse may have further rows."""
+    current, raw = _torch_current()
+    device = current()
+    rows, pages, width, batch = _chunk_shape("pgc_chunk_attn", device, q, k_pages, v_pages, block_tables, q_starts,
+                                             seq_lens, out, workspace, gate, lse)
     check(lib().pgc_chunk_attn(
-        _ptr(q), _ptr(k_pages), _ptr(v_pages), k_pages.shape[0], _ptr(block_tables), block_tables.shape[1],
-        _ptr(q_starts), _ptr(seq_lens), seq_lens.shape[0], q.shape[0], max_q_len, max_seq_len, scale, _ptr(gate),
-        _ptr(out), _ptr(lse), _ptr(workspace), workspace.numel() * workspace.element_size(), _stream(stream)),
-        "pgc_chunk_attn")
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, block_tables.data_ptr(), width, q_starts.data_ptr(),
+        seq_lens.data_ptr(), batch, rows, max_q_len, max_seq_len, scale, _ptr(gate), out.data_ptr(), _ptr(lse),
+        workspace.data_ptr(), workspace.nbytes, raw(device) if stream is None else _stream(stream)), "pgc_chunk_attn")
 
 
 def chunk_attn_weights(q, k_pages, v_pages, block_tables, q_starts, seq_lens, max_q_len, max_seq_len, scale,
                        out, weights, workspace, gate=None, lse=None, slots=None, stream=None) -> None:
     """pgc_chunk_attn_weights: chunk_attn that also adds the attention every cached token received to
     weights fp32 [num_slots][4][stride]; slots [batch] int32."""
+    what = "pgc_chunk_attn_weights"
+    current, raw = _torch_current()
+    device = current()
+    rows, pages, width, batch = _chunk_shape(what, device, q, k_pages, v_pages, block_tables, q_starts, seq_lens, out,
+                                             workspace, gate, lse)
+    _, i32, f32 = _dtypes()
+    num_slots, _, stride = _dims(what, "weights", weights, None, NUM_KV_HEADS, None)
+    _refuse(what, ("weights", weights, f32, 0, False), ("slots", slots, i32, 4 * batch, False))
     check(lib().pgc_chunk_attn_weights(
-        _ptr(q), _ptr(k_pages), _ptr(v_pages), k_pages.shape[0], _ptr(block_tables), block_tables.shape[1],
-        _ptr(q_starts), _ptr(seq_lens), seq_lens.shape[0], q.shape[0], max_q_len, max_seq_len, scale, _ptr(gate),
-        _ptr(out), _ptr(lse), _ptr(weights), weights.shape[2], weights.shape[0], _ptr(slots), _ptr(workspace),
-        workspace.numel() * workspace.element_size(), _stream(stream)), "pgc_chunk_attn_weights")
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, block_tables.data_ptr(), width, q_starts.data_ptr(),
+        seq_lens.data_ptr(), batch, rows, max_q_len, max_seq_len, scale, _ptr(gate), out.data_ptr(), _ptr(lse),
+        weights.data_ptr(), stride, num_slots, _ptr(slots), workspace.data_ptr(), workspace.nbytes,
+        raw(device) if stream is None else _stream(stream)), what)
 
 
 def kv_evict_select(weights, seq_lens, max_seq_len, budget, keep_first, keep_last, kept, new_lens=None,
                     weights_out=None, slots=None, stream=None) -> None:
-    """pgc_kv_evict_select: kept int32 [batch][4][budget] from weights fp32 [num_slots][4][stride]."""
+    """pgc_kv_evict_select: kept int32 [batch][4][budget] from weights fp32 [num_slots][4][stride]. All
+    contiguous and on the current device."""
+    what = "pgc_kv_evict_select"
+    current, raw = _torch_current()
+    device = current()
+    _, i32, f32 = _dtypes()
+    num_slots, heads, stride = weights.shape if weights.ndim == 3 else (0, 0, 0)
+    batch = seq_lens.shape[0]
+    kept_bytes, weight_bytes = batch * NUM_KV_HEADS * budget * 4, num_slots * NUM_KV_HEADS * stride * 4
+    if not (heads == NUM_KV_HEADS and weights.nbytes == weight_bytes and kept.nbytes == kept_bytes
+            and seq_lens.nbytes == 4 * batch and weights.dtype in f32
+            and weights.is_contiguous() and kept.is_contiguous() and seq_lens.is_contiguous()
+            and device == weights.get_device() == kept.get_device() == seq_lens.get_device()
+            and (weights_out is None or (weights_out.nbytes == weight_bytes and weights_out.is_contiguous()
+                                         and weights_out.get_device() == device))
+            and (new_lens is None or (new_lens.nbytes == 4 * batch and new_lens.is_contiguous() and new_lens.get_device() == device))
+            and (slots is None or (slots.nbytes == 4 * batch and slots.is_contiguous() and slots.get_device() == device))):
+        _dims(what, "weights", weights, None, NUM_KV_HEADS, None)
+        _dims(what, "seq_lens", seq_lens, None)
+        _refuse(what, ("weights", weights, f32, 0, False), ("weights_out", weights_out, f32, weight_bytes, True),
+                ("slots", slots, i32, 4 * batch, False), ("seq_lens", seq_lens, i32, 4 * batch, True),
+                ("kept", kept, i32, kept_bytes, True), ("new_lens", new_lens, i32, 4 * batch, False))
     check(lib().pgc_kv_evict_select(
-        _ptr(weights), _ptr(weights_out), weights.shape[2], weights.shape[0], _ptr(slots), _ptr(seq_lens),
-        seq_lens.shape[0], max_seq_len, budget, keep_first, keep_last, _ptr(kept), _ptr(new_lens),
-        _stream(stream)), "pgc_kv_evict_select")
+        weights.data_ptr(), _ptr(weights_out), stride, num_slots, _ptr(slots), seq_lens.data_ptr(), batch, max_seq_len,
+        budget, keep_first, keep_last, kept.data_ptr(), _ptr(new_lens), raw(device) if stream is None else _stream(stream)),
+        what)
 
 
 def kv_evict_compact(src_k, src_v, src_tables, kept, dst_k, dst_v, dst_tables, stream=None) -> None:
-    """pgc_kv_evict_compact: the rows kept int32 [batch][4][budget] into the pages of dst_tables."""
+    """pgc_kv_evict_compact: the rows kept int32 [batch][4][budget] into the pages of dst_tables. All
+    contiguous and on the current device."""
+    what = "pgc_kv_evict_compact"
+    current, raw = _torch_current()
+    device = current()
+    b16, i32, _ = _dtypes()
+    batch, heads, budget = kept.shape if kept.ndim == 3 else (0, 0, 0)
+    src_rows, src_width = src_tables.shape if src_tables.ndim == 2 else (-1, 0)
+    dst_rows, dst_width = dst_tables.shape if dst_tables.ndim == 2 else (-1, 0)
+    src_pages, dst_pages = src_k.shape[0], dst_k.shape[0]
+    src_bytes, dst_bytes = src_pages * _POOL_PAGE, dst_pages * _POOL_PAGE
+    if not (heads == NUM_KV_HEADS and src_rows >= batch and dst_rows >= batch
+            and src_k.nbytes == src_v.nbytes == src_bytes and dst_k.nbytes == dst_v.nbytes == dst_bytes
+            and kept.nbytes == 4 * batch * NUM_KV_HEADS * budget and src_tables.nbytes == 4 * src_rows * src_width
+            and dst_tables.nbytes == 4 * dst_rows * dst_width and src_k.dtype in b16 and dst_k.dtype in b16
+            and src_k.is_contiguous() and src_v.is_contiguous() and dst_k.is_contiguous() and dst_v.is_contiguous()
+            and kept.is_contiguous() and src_tables.is_contiguous() and dst_tables.is_contiguous()
+            and device == src_k.get_device() == src_v.get_device() == dst_k.get_device() == dst_v.get_device()
+            == kept.get_device() == src_tables.get_device() == dst_tables.get_device()):
+        _dims(what, "kept", kept, None, NUM_KV_HEADS, None)
+        _dims(what, "src_tables", src_tables, None, None)
+        _dims(what, "dst_tables", dst_tables, None, None)
+        _refuse(what, ("src_k", src_k, b16, src_bytes, True), ("src_v", src_v, b16, src_bytes, True),
+                ("src_tables", src_tables, i32, 4 * batch * src_width, False), ("kept", kept, i32, 0, False),
+                ("dst_k", dst_k, b16, dst_bytes, True), ("dst_v", dst_v, b16, dst_bytes, True),
+                ("dst_tables", dst_tables, i32, 4 * batch * dst_width, False))
     check(lib().pgc_kv_evict_compact(
-        _ptr(src_k), _ptr(src_v), src_k.shape[0], _ptr(src_tables), src_tables.shape[1], _ptr(kept),
-        kept.shape[0], kept.shape[2], _ptr(dst_k), _ptr(dst_v), dst_k.shape[0], _ptr(dst_tables),
-        dst_tables.shape[1], _stream(stream)), "pgc_kv_evict_compact")
+        src_k.data_ptr(), src_v.data_ptr(), src_pages, src_tables.data_ptr(), src_width, kept.data_ptr(), batch, budget,
+        dst_k.data_ptr(), dst_v.data_ptr(), dst_pages, dst_tables.data_ptr(), dst_width,
+        raw(device) if stream is None else _stream(stream)), what)
 
 
 def copy_rows(dst, src, n_rows, row_bytes, dst_pitch, src_pitch, dst_rows=None, src_rows=None,
