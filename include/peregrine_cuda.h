@@ -248,10 +248,12 @@ int pgc_prefill_attn(const uint16_t *q, const uint16_t *k_pages, const uint16_t 
 #define PGC_CHUNK_MAX_ROWS (1 << 22)   /* query rows of a call */
 #define PGC_CHUNK_MAX_TOKENS (1 << 24) /* tokens of a sequence */
 
-/* Workspace bytes of pgc_chunk_attn (with_weights = 0) and pgc_chunk_attn_weights (1). Up to
- * PGC_MAX_QUERIES rows a sequence: the splits' partials, and with weights 16 fp32 scores per query
- * row and token of max_seq_len; more rows: 38 MiB; with weights the rows' lse too. 0 for shapes that
- * the entries refuse. */
+/* Workspace bytes of pgc_chunk_attn (with_weights = 0) and pgc_chunk_attn_weights (1): the partials of cut
+ * units, some 9 MiB at 4 rows a sequence and less for fewer, 38 MiB for more than PGC_MAX_QUERIES. With
+ * weights also 64 bytes a query row, and up to PGC_MAX_QUERIES rows a sequence the scores, 64 bytes a query row
+ * and token of max_seq_len, by the bound and not by the lengths: 16 single rows take 67 MB at a bound of 65536,
+ * 64 take 1.07 GB at 262144. A server whose bound makes that too much gives max_q_len = 5, which needs no
+ * scores (and takes the form for chunks). 0 for shapes that the entries refuse. */
 size_t pgc_chunk_workspace_bytes(int batch, int total_q, int max_q_len, int max_seq_len,
                                  int with_weights);
 

@@ -9,12 +9,14 @@
 //
 // Forms, chosen by the host bounds:
 //   * up to PGC_MAX_QUERIES rows a sequence: chunk_split_kernel (mma.sync), bound by the K/V bytes (64
-//     sequences of 1024 to 32768 tokens, 2.1 GB: 323 us, 6.5 TB/s); with weights it leaves the scores in
+//     sequences of 1024 to 32768 tokens, 2.1 GB: 333 us, 6.3 TB/s); with weights it leaves the scores in
 //     the workspace, 16 B per row, kv head and token beside 1 KiB of K and V, so that K is read once.
-//     Few short sequences take its cluster form, bound by latency (one row over 4097 tokens: 10.7 us,
-//     over 500: 7.0);
-//   * more rows: chunk_pair_kernel on the 5th-gen tensor cores (1600 tokens over 24576: 463 us, 1440
+//     Few short sequences take its cluster form, bound by latency (one row over 4097 tokens: 10.3 us,
+//     over 500: 6.6);
+//   * more rows: chunk_pair_kernel on the 5th-gen tensor cores (1600 tokens over 24576: 540 us, 1230
 //     TFLOP/s), and chunk_weights.cu for the weights.
+// These are medians of calls behind one another; the first ones, before the power cap lowers the clock, take
+// 323 us and 464 (1430 TFLOP/s). Comparisons of large calls below were taken in such short bursts.
 // But for the cluster form, the line of all the batch's tiles is cut into equal consecutive shares, one
 // per CTA (or pair) of a fixed grid: lengths are on the device, and a grid by the host's bounds would be
 // empty for the most part where they are ragged (387 us for the 64 sequences above). A unit of work cut by
@@ -1693,7 +1695,8 @@ __global__ void __launch_bounds__(kFinishThreads) chunk_finish_kernel(const Fini
 // The split form's cluster form: its launch, and the CTAs of a cluster (0: the line form is to be taken). A
 // short batch is bound by latency, which the cluster form has less of (one launch); but it takes the
 // sequences as they are, so it is for batches whose clusters all run at once, and up to kClusterTokens a
-// CTA. One row, us: 500 tokens 7.0 against 12.8 of the line form, 4097 10.6 against 15.8, 16000 21.5 against
+// CTA. Bounds count, not lengths: a call that is to be replayed with up to 65536 tokens takes the line form.
+// One row, us: 500 tokens 7.0 against 12.8 of the line form, 4097 10.6 against 15.8, 16000 21.5 against
 // 22.5, 32768 36.8 against 33.1; 8 sequences of 1000 9.9 against 15.7, 37 of 300 13.5 against 21.2. Where the
 // clusters took two turns: 4 sequences of 300, 8 CTAs each, 11.9 against 12.9, of 2000 16.3 against 16.2.
 constexpr int kClusterTokens = 512;
